@@ -3,6 +3,9 @@
 Public surface, as in the reference (chroma/__init__.py:14-26): ``compile``, ``Program``, ``Decoder``; plus
 ``BatchDecoder`` for device-resident batched decoding. Loading and running artefacts needs NumPy only; ``compile``
 imports Torch on first use.
+
+Operators for serving over a paged key-value cache, on CUDA tensors: ``paged_append``, ``paged_attention``,
+``step_pages``, ``compact_pages``, and ``process_logits`` for the logits that follow.
 """
 
 from __future__ import annotations
@@ -32,4 +35,20 @@ def compile_model(model: Any, output: str | Path, *, steps: int, context: int | 
     return _compile_model(model, output, steps=steps, context=context, last=last, experts=experts)
 
 
-__all__ = ["BatchDecoder", "Decoder", "ExpertGroup", "Program", "compile", "compile_model"]
+# Operators on CUDA tensors of the caller (a paged key-value cache, its attention, logits): Torch is imported by the
+# caller, who has the tensors.
+_OPERATORS = {"paged_append": "paged", "paged_attention": "paged", "step_pages": "paged", "compact_pages": "paged",
+              "process_logits": "logits"}
+
+
+def __getattr__(name: str) -> Any:
+    if name in _OPERATORS:
+        from importlib import import_module
+
+        value = getattr(import_module(f"chroma_b200._src.{_OPERATORS[name]}"), name)
+        globals()[name] = value
+        return value
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+__all__ = ["BatchDecoder", "Decoder", "ExpertGroup", "Program", "compile", "compile_model", *_OPERATORS]

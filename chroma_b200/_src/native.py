@@ -104,6 +104,14 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "chroma_b200_graph_device": (ctypes.c_char_p, [_VP]),
     "chroma_b200_graph_launches": (ctypes.c_int32, [_VP]),
     "chroma_b200_graph_destroy": (None, [_VP]),
+    "chroma_b200_paged_append": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _I32, _VP, _CP, _SZ]),
+    "chroma_b200_paged_attention": (ctypes.c_int, [_VP, _VP, _VP, _CP, _SZ]),
+    "chroma_b200_attention_workspace": (ctypes.c_int64, [_I32, _I32, _I32, _I32]),
+    "chroma_b200_step_pages": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_int64, _VP, _CP, _SZ]),
+    "chroma_b200_compact_pages": (ctypes.c_int, [_VP, _VP, _VP, _VP, ctypes.c_int64, _VP, _CP, _SZ]),
+    "chroma_b200_pages_workspace": (ctypes.c_int64, [_I32, _I32]),
+    "chroma_b200_process_logits": (ctypes.c_int, [_VP, _VP, _CP, _SZ]),
+    "chroma_b200_logits_workspace": (ctypes.c_int64, [_I32, _I32]),
 }
 
 EP_HANDLE_BYTES = 64  # CHROMA_B200_EP_HANDLE_BYTES
@@ -142,6 +150,19 @@ _ERRORS = {INDEX: IndexError, VALUE: ValueError, RUNTIME: RuntimeError}
 def call(name: str, *args: Any) -> None:
     err = ctypes.create_string_buffer(1024)
     status = getattr(lib(), name)(*args, err, len(err))
+    if status != OK:
+        raise _ERRORS.get(status, RuntimeError)(err.value.decode(errors="replace") or name)
+
+
+_local = threading.local()
+
+
+def call_op(name: str, *args: Any) -> None:
+    """``call`` for operators that run every few microseconds: one message buffer per thread."""
+    err = getattr(_local, "err", None)
+    if err is None:
+        err = _local.err = ctypes.create_string_buffer(1024)
+    status = getattr(_lib or lib(), name)(*args, err, 1024)
     if status != OK:
         raise _ERRORS.get(status, RuntimeError)(err.value.decode(errors="replace") or name)
 

@@ -14,7 +14,7 @@ from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
 ROOT = PACKAGE.parent
-SOURCES = [PACKAGE / "csrc" / "runtime.cu", PACKAGE / "csrc" / "graph.cu"]
+SOURCES = [PACKAGE / "csrc" / "runtime.cu", PACKAGE / "csrc" / "graph.cu", PACKAGE / "csrc" / "ops.cu"]
 DEPENDS = sorted((PACKAGE / "csrc").glob("*.cu*")) + [ROOT / "include" / "chroma_b200.h"]
 TARGET = PACKAGE / "libchroma_b200.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -28,7 +28,7 @@ def nvcc() -> str:
 
 
 def command(target: Path = TARGET) -> list[str]:
-    return [nvcc(), "-O3", "-std=c++17", *ARCH, "-lineinfo", "-Xcompiler", "-fPIC", "-shared", "--cudart=static",
+    return [nvcc(), "-O3", "-std=c++17", *ARCH, "-lineinfo", "-Xcompiler", "-fPIC", "-shared", "--cudart=static", "--threads", "0",
             "-I", str(ROOT / "include"), *map(str, SOURCES), "-o", str(target)]
 
 

@@ -115,7 +115,7 @@ __device__ __forceinline__ void prefetch_l2(const void* p, size_t bytes, int lan
 }
 
 // Grid-stride L2 prefetch of a byte range (one 128-byte line per thread step).
-__global__ void k_prefetch_l2(const char* base, size_t bytes) {
+[[maybe_unused]] static __global__ void k_prefetch_l2(const char* base, size_t bytes) {
     const size_t lines = (bytes + 127) / 128;
     for (size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x; i < lines; i += size_t(gridDim.x) * blockDim.x)
         asm volatile("prefetch.global.L2 [%0];" ::"l"(base + i * 128));
@@ -128,7 +128,7 @@ __device__ __forceinline__ void bulk_prefetch_l2(const void* p, unsigned bytes) 
 }
 
 // Grid-stride bulk L2 prefetch of a 16-byte aligned range in 64 KiB pieces (one thread per piece).
-__global__ void k_prefetch_l2_bulk(const char* base, size_t bytes) {
+[[maybe_unused]] static __global__ void k_prefetch_l2_bulk(const char* base, size_t bytes) {
     constexpr size_t kPiece = 64 * 1024;
     const size_t pieces = (bytes + kPiece - 1) / kPiece;
     for (size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x; i < pieces; i += size_t(gridDim.x) * blockDim.x) {

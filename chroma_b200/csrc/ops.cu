@@ -1,0 +1,242 @@
+// C entries of the operators over a paged key-value cache and of logits processing (include/chroma_b200.h): checks of
+// their arguments, choice of kernel, launches. Nothing here allocates or synchronises.
+#include "../../include/chroma_b200.h"
+
+#include <cstdio>
+#include <stdexcept>
+#include <string>
+#include <utility>
+
+#include "logits.cuh"
+#include "paged.cuh"
+#include "pages.cuh"
+
+namespace {
+
+using namespace cb200;
+
+struct OpsValueError : std::runtime_error { using std::runtime_error::runtime_error; };
+
+template <typename F> int guarded_op(char* err, size_t n, F&& f) {
+    const char* text = "unknown native error";
+    int code = CHROMA_B200_RUNTIME;
+    std::string held;
+    try {
+        f();
+        return CHROMA_B200_OK;
+    } catch (const OpsValueError& e) {
+        code = CHROMA_B200_VALUE;
+        held = e.what();
+        text = held.c_str();
+    } catch (const std::exception& e) {
+        held = e.what();
+        text = held.c_str();
+    } catch (...) {
+    }
+    if (err && n) std::snprintf(err, n, "%s", text);
+    return code;
+}
+
+void want(bool ok, const char* what) {
+    if (!ok) throw OpsValueError(what);
+}
+
+void check(cudaError_t status, const char* what) {
+    if (status != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(status));
+}
+
+template <typename... Params, typename... Args>
+void launch(cudaStream_t s, dim3 grid, dim3 block, size_t smem, void (*kernel)(Params...), Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    check(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...), "kernel launch");
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+constexpr int kMaxRows = 1 << 30;  // positions of a slot: row numbers stay well inside 32 bits
+
+size_t element(int storage) { return storage == CHROMA_B200_BF16 ? 2 : 4; }
+
+void check_pages(const chroma_b200_pages* p) {
+    want(p && p->keys && p->values && p->table && p->lengths, "null argument");
+    want(p->storage == CHROMA_B200_FP32 || p->storage == CHROMA_B200_BF16, "pools are fp32 or bf16");
+    want(p->layers > 0 && p->pages > 0 && p->page_rows > 0 && p->kv_heads > 0 && p->slots > 0 && p->width > 0,
+         "empty pool or table");
+    const int64_t size = int64_t(element(p->storage));
+    want(p->head_dim > 0 && p->head_dim * size % 16 == 0 && p->head_dim <= 128,
+         "head_dim: at most 128, and a multiple of 16 bytes");
+    want(int64_t(p->width) * p->page_rows <= kMaxRows, "a table of more than 2^30 positions");
+    want(aligned16(p->keys) && aligned16(p->values), "pools must be 16-byte aligned");
+    for (int i = 0; i < 4; ++i)
+        want(p->key_strides[i] * size % 16 == 0 && p->value_strides[i] * size % 16 == 0,
+             "strides of the pools must be multiples of 16 bytes");
+}
+
+template <typename F> void by_type(int storage, F&& f) {
+    if (storage == CHROMA_B200_BF16) f(__nv_bfloat16());
+    else f(float());
+}
+
+PoolArgs pool_args(const chroma_b200_pages& p) {
+    const int64_t per = 16 / int64_t(element(p.storage));
+    PoolArgs a{};
+    a.k = static_cast<uint4*>(p.keys);
+    a.v = static_cast<uint4*>(p.values);
+    a.kl = p.key_strides[0] / per, a.kp = p.key_strides[1] / per, a.kr = p.key_strides[2] / per, a.kh = p.key_strides[3] / per;
+    a.vl = p.value_strides[0] / per, a.vp = p.value_strides[1] / per, a.vr = p.value_strides[2] / per, a.vh = p.value_strides[3] / per;
+    a.layers = p.layers;
+    a.heads = p.kv_heads;
+    a.run = int(p.head_dim / per);
+    return a;
+}
+
+dim3 table_grid(const chroma_b200_pages& p) { return dim3(unsigned((p.width + 255) / 256), unsigned(p.slots)); }
+
+}  // namespace
+
+extern "C" {
+
+int chroma_b200_paged_append(const chroma_b200_pages* p, const void* new_keys, const void* new_values,
+                             const int64_t* new_strides, const int32_t* starts, int32_t tokens, void* stream, char* err,
+                             size_t err_len) {
+    return guarded_op(err, err_len, [&] {
+        check_pages(p);
+        want(tokens >= 0 && new_strides, "null argument");
+        want(starts || tokens == p->slots, "without starts there is one row per slot");
+        if (!tokens) return;
+        want(new_keys && new_values, "null argument");
+        AppendArgs a{};
+        a.nk = new_keys, a.nv = new_values;
+        a.nkt = new_strides[0], a.nkh = new_strides[1], a.nvt = new_strides[2], a.nvh = new_strides[3];
+        a.k = p->keys, a.v = p->values;
+        a.kp = p->key_strides[1], a.kr = p->key_strides[2], a.kh = p->key_strides[3];
+        a.vp = p->value_strides[1], a.vr = p->value_strides[2], a.vh = p->value_strides[3];
+        a.table = p->table, a.ts = p->table_stride, a.lengths = p->lengths, a.starts = starts;
+        a.slots = p->slots, a.width = p->width, a.pages = p->pages, a.page = p->page_rows, a.kv = p->kv_heads;
+        a.dim = p->head_dim, a.tokens = tokens, a.by_page = FastDiv(uint32_t(p->page_rows));
+        by_type(p->storage, [&](auto t) {
+            launch(cudaStream_t(stream), dim3(unsigned(tokens)), dim3(128), 0, k_paged_append<decltype(t)>, a);
+        });
+    });
+}
+
+int64_t chroma_b200_attention_workspace(int32_t, int32_t, int32_t, int32_t) { return 0; }
+
+int chroma_b200_paged_attention(const chroma_b200_pages* p, const chroma_b200_attention* g, void* stream, char* err,
+                                size_t err_len) {
+    return guarded_op(err, err_len, [&] {
+        check_pages(p);
+        want(g && g->tokens >= 0, "null argument");
+        want(g->heads > 0 && g->heads % p->kv_heads == 0, "heads must be a multiple of kv_heads");
+        want(g->starts || g->tokens == p->slots, "without starts there is one token per slot");
+        want(g->first >= 0, "first must be nonnegative");
+        want(int64_t(g->tokens) * g->heads <= kMaxRows, "more than 2^30 rows of queries");
+        if (!g->tokens) return;
+        want(g->q && g->out, "null argument");
+        PagedArgs a{};
+        a.k = p->keys, a.v = p->values;
+        a.kp = p->key_strides[1], a.kr = p->key_strides[2], a.kh = p->key_strides[3];
+        a.vp = p->value_strides[1], a.vr = p->value_strides[2], a.vh = p->value_strides[3];
+        a.table = p->table, a.ts = p->table_stride, a.lengths = p->lengths, a.starts = g->starts;
+        a.slots = p->slots, a.width = p->width, a.pages = p->pages, a.page = p->page_rows, a.kv = p->kv_heads;
+        a.dim = p->head_dim, a.by_page = FastDiv(uint32_t(p->page_rows));
+        a.q = g->q, a.out = g->out, a.lse = g->lse, a.sinks = g->sinks, a.sinks_fp32 = g->sinks_fp32;
+        a.qt = g->q_strides[0], a.qh = g->q_strides[1], a.ot = g->out_strides[0], a.oh = g->out_strides[1];
+        a.tokens = g->tokens, a.heads = g->heads, a.group = g->heads / p->kv_heads;
+        a.window = g->window, a.first = g->first, a.scale_log2 = g->scale * kLog2e;
+        const int64_t rows = int64_t(g->tokens) * g->heads;
+        by_type(p->storage, [&](auto t) {
+            launch(cudaStream_t(stream), dim3(unsigned((rows + 3) / 4)), dim3(128), size_t(16) * p->head_dim,
+                   k_paged_attention_rows<decltype(t)>, a);
+        });
+    });
+}
+
+int64_t chroma_b200_pages_workspace(int32_t pages, int32_t slots) {
+    return pages < 0 || slots < 0 ? -1 : (5 * int64_t(pages) + 3 * int64_t(slots) + 4) * 4;
+}
+
+int chroma_b200_step_pages(const chroma_b200_pages* p, const int32_t* parents, const int32_t* counts, int32_t* new_table,
+                           int32_t* new_lengths, int32_t* info, void* workspace, int64_t workspace_bytes, void* stream,
+                           char* err, size_t err_len) {
+    return guarded_op(err, err_len, [&] {
+        check_pages(p);
+        want(parents && counts && new_table && new_lengths && info && workspace, "null argument");
+        want(workspace_bytes >= chroma_b200_pages_workspace(p->pages, p->slots), "workspace too small");
+        want((int64_t(p->page_rows) + 1) * p->slots < (int64_t(1) << 32), "page_rows * slots must be below 2^32");
+        want(p->slots <= 65535, "at most 65,535 slots");
+        const auto s = cudaStream_t(stream);
+        StepArgs a{};
+        a.table = p->table, a.ts = p->table_stride, a.lengths = p->lengths, a.parents = parents, a.counts = counts;
+        a.new_table = new_table, a.new_lengths = new_lengths, a.info = info;
+        a.keeper = static_cast<unsigned*>(workspace);
+        a.free_list = static_cast<int*>(workspace) + p->pages;
+        a.copies = a.free_list + p->pages;
+        a.slots = p->slots, a.width = p->width, a.pages = p->pages, a.page = p->page_rows;
+        check(cudaMemsetAsync(a.keeper, 0, size_t(p->pages) * 4, s), "memset");
+        launch(s, table_grid(*p), dim3(256), 0, k_pages_gather, a);
+        launch(s, dim3(1), dim3(1024), 0, k_pages_assign, a);
+        launch(s, dim3(592), dim3(256), 0, k_pages_copy, pool_args(*p), a.copies, a.copies + 3 * p->slots);
+    });
+}
+
+int chroma_b200_compact_pages(const chroma_b200_pages* p, int32_t* new_table, int32_t* info, void* workspace,
+                              int64_t workspace_bytes, void* stream, char* err, size_t err_len) {
+    return guarded_op(err, err_len, [&] {
+        check_pages(p);
+        want(new_table && info && workspace, "null argument");
+        want(workspace_bytes >= chroma_b200_pages_workspace(p->pages, p->slots), "workspace too small");
+        want(p->slots <= 65535, "at most 65,535 slots");
+        const auto s = cudaStream_t(stream);
+        CompactArgs a{};
+        a.table = p->table, a.ts = p->table_stride, a.lengths = p->lengths;
+        a.new_table = new_table, a.info = info;
+        a.held = static_cast<unsigned*>(workspace);
+        a.to = static_cast<int*>(workspace) + p->pages;
+        a.copies = a.to + p->pages;
+        a.slots = p->slots, a.width = p->width, a.pages = p->pages, a.page = p->page_rows;
+        check(cudaMemsetAsync(a.held, 0, size_t(p->pages) * 4, s), "memset");
+        launch(s, table_grid(*p), dim3(256), 0, k_compact_mark, a);
+        launch(s, dim3(1), dim3(1024), 0, k_compact_plan, a);
+        launch(s, dim3(1184), dim3(256), 0, k_pages_copy, pool_args(*p), a.copies, a.copies + 3 * p->pages);
+        launch(s, table_grid(*p), dim3(256), 0, k_compact_table, a);
+    });
+}
+
+int64_t chroma_b200_logits_workspace(int32_t rows, int32_t vocab) {
+    return rows < 0 || vocab < 0 ? -1 : int64_t(rows) * ((vocab + kLogitsSegment - 1) / kLogitsSegment) * 8;
+}
+
+int chroma_b200_process_logits(const chroma_b200_logits* g, void* stream, char* err, size_t err_len) {
+    return guarded_op(err, err_len, [&] {
+        want(g && g->rows >= 0 && g->vocab > 0 && g->vocab <= kMaxRows, "null argument or empty vocabulary");
+        want(g->storage == CHROMA_B200_FP32 || g->storage == CHROMA_B200_BF16, "logits are fp32 or bf16");
+        want(!g->history || (g->lengths && g->width >= 0), "a history needs its lengths");
+        want(!g->bias_ids || (g->bias && g->biases >= 0), "bias_ids need their bias");
+        want(g->rows <= 65535, "at most 65,535 rows");
+        if (!g->rows) return;
+        want(g->logits && g->out, "null argument");
+        want(!g->argmax || (g->workspace && g->workspace_bytes >= chroma_b200_logits_workspace(g->rows, g->vocab)),
+             "workspace too small");
+        const auto s = cudaStream_t(stream);
+        LogitsArgs a{};
+        a.logits = g->logits, a.out = g->out, a.history = g->history, a.lengths = g->lengths, a.prompts = g->prompts;
+        a.repetition = g->repetition, a.presence = g->presence, a.frequency = g->frequency, a.temperature = g->temperature;
+        a.bias_ids = g->bias_ids, a.bias = g->bias, a.mask = reinterpret_cast<const unsigned*>(g->mask);
+        a.best = g->argmax ? static_cast<unsigned long long*>(g->workspace) : nullptr;
+        a.stride = g->stride, a.out_stride = g->out_stride, a.history_stride = g->history_stride;
+        a.bias_ids_stride = g->bias_ids_stride, a.bias_stride = g->bias_stride, a.mask_stride = g->mask_stride;
+        a.vocab = g->vocab, a.width = g->width, a.biases = g->biases;
+        a.segments = (g->vocab + kLogitsSegment - 1) / kLogitsSegment;
+        by_type(g->storage, [&](auto t) {
+            launch(s, dim3(unsigned(a.segments), unsigned(g->rows)), dim3(256), 0, k_logits<decltype(t)>, a);
+        });
+        if (g->argmax) launch(s, dim3(unsigned(g->rows)), dim3(32), 0, k_logits_pick, a.best, a.segments, g->argmax);
+    });
+}
+
+}  // extern "C"

@@ -233,6 +233,98 @@ void chroma_b200_ep_destroy(chroma_b200_ep* ep);
 int chroma_b200_create_ep(const chroma_b200_desc* desc, const char* weights_path, const void* device_weights,
                           chroma_b200_ep* ep, chroma_b200_program** out, char* err, size_t err_len);
 
+/* ---- Operators over a paged key-value cache ----------------------------------------------------------------------
+ * No reference counterpart: the reference's cache is one contiguous block per Program (chroma/_src/decoder.py:44-152).
+ * Here a cache is two pools of pages that sequences share, a table with the pages of each sequence, and the number of
+ * rows each holds. All pointers are device pointers of the current device; the calls are queued on `stream` (a
+ * cudaStream_t) and allocate nothing. Position p of slot s is row p % page_rows of page table[s][p / page_rows].
+ * Table entries below 0 or beyond the pool name no page: their positions are never seen, written or copied. */
+typedef struct chroma_b200_pages {
+    void *keys, *values;          /* [layers][pages][page_rows][kv_heads][head_dim] in `storage` */
+    const int32_t *table;         /* [slots][width], rows `table_stride` apart */
+    const int32_t *lengths;       /* [slots] rows held, the rows that the call appends or queries included */
+    int64_t key_strides[4];       /* elements between layers, pages, rows, heads; a head's row is contiguous */
+    int64_t value_strides[4];
+    int64_t table_stride;
+    int32_t storage;              /* CHROMA_B200_FP32 / CHROMA_B200_BF16 */
+    int32_t layers, pages, page_rows, kv_heads, head_dim, slots, width;
+} chroma_b200_pages;
+
+/* Head rows are multiples of 16 bytes (head_dim a multiple of 8 in bf16, of 4 in fp32), pools and their strides
+ * 16-byte aligned. */
+
+/* Writes new rows into the pages that already belong to their sequences: row i of slot b (rows starts[b] to
+ * starts[b + 1]; row b alone where `starts` is NULL) goes to position lengths[b] - rows + i. Layer 0 of the pools.
+ * new_strides: elements between tokens and heads of new_keys, then of new_values. */
+int chroma_b200_paged_append(const chroma_b200_pages* pages, const void* new_keys, const void* new_values,
+                             const int64_t* new_strides, const int32_t* starts, int32_t tokens, void* stream, char* err,
+                             size_t err_len);
+
+typedef struct chroma_b200_attention {
+    const void *q;                /* [tokens][heads][head_dim] in the pools' storage */
+    void *out;                    /* the same shape and type */
+    float *lse;                   /* [tokens][heads] or NULL */
+    const void *sinks;            /* [heads] or NULL: one more term of the softmax's sum, with no value */
+    const int32_t *starts;        /* [slots + 1], or NULL: one token per slot */
+    void *workspace;              /* chroma_b200_attention_workspace bytes */
+    int64_t workspace_bytes;
+    int64_t q_strides[2];         /* elements between tokens, heads */
+    int64_t out_strides[2];
+    int32_t tokens, heads;
+    int32_t sinks_fp32;           /* 1: fp32 sinks, 0: the pools' storage */
+    int32_t window, first;        /* window <= 0: none */
+    float scale;
+} chroma_b200_attention;
+
+/* out = softmax(scale q.K^T) V of each token over the positions it sees. Token i of slot b is at position
+ * p = lengths[b] - tokens of b + i and sees j <= p with p - j < window or j < first. The attention of
+ * chroma/models/gpt_oss.py:133-151 (learned sinks, sliding window) over pages; `lse` is the logarithm of the sum. A
+ * token that sees nothing gives zeros, and its sink (or -inf) as lse. */
+int chroma_b200_paged_attention(const chroma_b200_pages* pages, const chroma_b200_attention* args, void* stream,
+                                char* err, size_t err_len);
+/* Bytes of workspace that paged_attention wants for these heads and this head_dim on the current device. */
+int64_t chroma_b200_attention_workspace(int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim);
+
+/* One step of a set of sequences. Slot s continues slot parents[s] (any slot may be continued by several; -1, or any
+ * other number that is no slot, empties s), and counts[s] more rows are reserved for it. Writes the new table
+ * [slots][width] (contiguous; entries past a slot's pages are -1), the new lengths, and info[3] = {pages left free,
+ * pages short, pages copied}. A page that no slot holds is free. Free pages are given out from the lowest number, to
+ * slots from the lowest. A slot that will write into a page which another slot holds too gets a copy of its rows (all
+ * layers) first; the holder with the most rows in that page, the lowest slot among equals, keeps it. With too few
+ * free pages the last entries stay -1; a length that passes width * page_rows is cut there. Neither output may be an
+ * input. `workspace`: chroma_b200_pages_workspace bytes. */
+int chroma_b200_step_pages(const chroma_b200_pages* pages, const int32_t* parents, const int32_t* counts,
+                           int32_t* new_table, int32_t* new_lengths, int32_t* info, void* workspace,
+                           int64_t workspace_bytes, void* stream, char* err, size_t err_len);
+/* Moves the n pages that slots hold to numbers below n: the i-th held page from n up goes to the i-th free page
+ * below n, all layers. Writes the new table [slots][width] (not the input's memory) and info[2] = {n, moved}. */
+int chroma_b200_compact_pages(const chroma_b200_pages* pages, int32_t* new_table, int32_t* info, void* workspace,
+                              int64_t workspace_bytes, void* stream, char* err, size_t err_len);
+int64_t chroma_b200_pages_workspace(int32_t pages, int32_t slots);
+
+typedef struct chroma_b200_logits {
+    const void *logits;           /* [rows][vocab], rows `stride` apart */
+    void *out;                    /* [rows][vocab], rows `out_stride` apart; may be `logits` */
+    int64_t *argmax;              /* [rows] or NULL: of what is written, the lowest index among equals */
+    const int32_t *history;       /* [rows][width] token ids, rows `history_stride` apart, or NULL */
+    const int32_t *lengths;       /* [rows] tokens of the history in use */
+    const int32_t *prompts;       /* [rows] how many of those are the prompt's, or NULL: none */
+    const float *repetition, *presence, *frequency, *temperature; /* [rows] each, or NULL */
+    const int32_t *bias_ids;      /* [rows][biases], or NULL */
+    const float *bias;            /* [rows][biases] */
+    const int32_t *mask;          /* [rows][(vocab + 31) / 32] bits, 1 = allowed, rows `mask_stride` apart, or NULL */
+    void *workspace;              /* with argmax: chroma_b200_logits_workspace bytes */
+    int64_t stride, out_stride, history_stride, bias_ids_stride, bias_stride, mask_stride, workspace_bytes;
+    int32_t storage, rows, vocab, width, biases;
+} chroma_b200_logits;
+
+/* l = logits; of a token that occurs in the history: l / repetition where l > 0, else l * repetition;
+ * l -= frequency * c + presence * (c > 0), c = occurrences after the prompt; l += the token's biases, in list order;
+ * l /= temperature (0: left as it is); -inf where the mask has a 0. In 32 bits, rounded once to the storage type.
+ * Token ids outside the vocabulary are ignored. */
+int chroma_b200_process_logits(const chroma_b200_logits* args, void* stream, char* err, size_t err_len);
+int64_t chroma_b200_logits_workspace(int32_t rows, int32_t vocab);
+
 #ifdef __cplusplus
 }
 #endif
