@@ -5,10 +5,12 @@
 #include <cstdio>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 #include <utility>
 
 #include "logits.cuh"
 #include "paged.cuh"
+#include "paged_decode.cuh"
 #include "pages.cuh"
 
 namespace {
@@ -55,6 +57,28 @@ void launch(cudaStream_t s, dim3 grid, dim3 block, size_t smem, void (*kernel)(P
     check(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...), "kernel launch");
 }
 
+// A kernel that may start while the one before it drains; it waits for that one's results itself.
+template <typename... Params, typename... Args>
+void launch_after(cudaStream_t s, dim3 grid, dim3 block, void (*kernel)(Params...), Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    check(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...), "kernel launch");
+}
+
+int sm_count() {
+    int device = 0, n = 0;
+    check(cudaGetDevice(&device), "device");
+    check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device), "device attribute");
+    return n;
+}
+
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 constexpr int kMaxRows = 1 << 30;  // positions of a slot: row numbers stay well inside 32 bits
@@ -94,6 +118,58 @@ PoolArgs pool_args(const chroma_b200_pages& p) {
     return a;
 }
 
+// Workspace of a decode: partial results of two items per CTA, and each CTA's join.
+struct DecodeSpace {
+    int grid, tiles, pad;  // CTAs, tiles of 8 heads in a block, padded head row
+    int64_t parts, ml, bytes;
+    DecodeSpace(int heads, int kv, int dim) {
+        const int group = heads / kv;
+        tiles = group > 8 ? 2 : 1;
+        pad = dim <= 32 ? 32 : dim <= 64 ? 64 : 128;
+        grid = sm_count() * (pad == 128 ? 1 : 2);
+        parts = int64_t(2) * grid * 8 * tiles * pad * 4;
+        ml = int64_t(2) * grid * 8 * tiles * 8;
+        bytes = parts + ml + int64_t(grid) * 16;
+    }
+};
+
+template <int DC, int NT> void decode_bf16(const PagedDecodeArgs& p, int grid, bool aligned, cudaStream_t s) {
+    const auto kernel = aligned ? k_paged_decode<DC, NT, true> : k_paged_decode<DC, NT, false>;
+    constexpr int smem = DecodeShape<DC>::kSmem;
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "smem attribute");
+    launch(s, dim3(unsigned(grid)), dim3(kDecThreads), smem, kernel, p);
+    if (!p.whole) launch_after(s, dim3(unsigned(grid), 8 * NT), dim3(128), k_paged_join<__nv_bfloat16, 32 * DC>, p, 8 * NT);
+}
+
+void decode(const PagedArgs& a, const chroma_b200_attention& g, int storage, cudaStream_t s) {
+    const DecodeSpace space(a.heads, a.kv, a.dim);
+    PagedDecodeArgs p{};
+    p.a = a;
+    p.blocks = (a.group + 8 * space.tiles - 1) / (8 * space.tiles);
+    const int64_t items = int64_t(a.slots) * a.kv * p.blocks;
+    // Short tables need no cut: at 1,024 positions an item is 8 units a warp. Neither do many items: they even out.
+    p.whole = int64_t(a.width) * a.page <= 1024 || items >= int64_t(16) * space.grid;
+    want(items < kMaxRows, "more than 2^30 heads");
+    p.least = 16;
+    const int64_t size = int64_t(element(storage));
+    p.q_vector = aligned16(a.q) && a.qt * size % 16 == 0 && a.qh * size % 16 == 0;
+    if (!p.whole) {
+        want(g.workspace && g.workspace_bytes >= space.bytes, "workspace too small");
+        p.parts = static_cast<float*>(g.workspace);
+        p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(g.workspace) + space.parts);
+        p.joins = reinterpret_cast<int4*>(static_cast<char*>(g.workspace) + space.parts + space.ml);
+    }
+    const int grid = p.whole ? int(items) : space.grid;
+    const bool aligned = a.page % 16 == 0;
+    const auto by_dim = [&](auto dc) {
+        if (space.tiles == 2) decode_bf16<decltype(dc)::value, 2>(p, grid, aligned, s);
+        else decode_bf16<decltype(dc)::value, 1>(p, grid, aligned, s);
+    };
+    if (space.pad == 32) by_dim(std::integral_constant<int, 1>());
+    else if (space.pad == 64) by_dim(std::integral_constant<int, 2>());
+    else by_dim(std::integral_constant<int, 4>());
+}
+
 dim3 table_grid(const chroma_b200_pages& p) { return dim3(unsigned((p.width + 255) / 256), unsigned(p.slots)); }
 
 }  // namespace
@@ -124,7 +200,14 @@ int chroma_b200_paged_append(const chroma_b200_pages* p, const void* new_keys, c
     });
 }
 
-int64_t chroma_b200_attention_workspace(int32_t, int32_t, int32_t, int32_t) { return 0; }
+int64_t chroma_b200_attention_workspace(int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim) {
+    if (tokens < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return -1;
+    try {
+        return DecodeSpace(heads, kv_heads, head_dim).bytes;
+    } catch (...) {
+        return -1;
+    }
+}
 
 int chroma_b200_paged_attention(const chroma_b200_pages* p, const chroma_b200_attention* g, void* stream, char* err,
                                 size_t err_len) {
@@ -149,6 +232,7 @@ int chroma_b200_paged_attention(const chroma_b200_pages* p, const chroma_b200_at
         a.tokens = g->tokens, a.heads = g->heads, a.group = g->heads / p->kv_heads;
         a.window = g->window, a.first = g->first, a.scale_log2 = g->scale * kLog2e;
         const int64_t rows = int64_t(g->tokens) * g->heads;
+        if (!g->starts && p->storage == CHROMA_B200_BF16) return decode(a, *g, p->storage, cudaStream_t(stream));
         by_type(p->storage, [&](auto t) {
             launch(cudaStream_t(stream), dim3(unsigned((rows + 3) / 4)), dim3(128), size_t(16) * p->head_dim,
                    k_paged_attention_rows<decltype(t)>, a);
