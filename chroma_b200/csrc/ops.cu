@@ -135,9 +135,7 @@ struct DecodeSpace {
 
 template <int DC, int NT> void decode_bf16(const PagedDecodeArgs& p, int grid, bool aligned, cudaStream_t s) {
     const auto kernel = aligned ? k_paged_decode<DC, NT, true> : k_paged_decode<DC, NT, false>;
-    constexpr int smem = DecodeShape<DC>::kSmem;
-    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "smem attribute");
-    launch(s, dim3(unsigned(grid)), dim3(kDecThreads), smem, kernel, p);
+    launch(s, dim3(unsigned(grid)), dim3(kDecThreads), 0, kernel, p);
     if (!p.whole) launch_after(s, dim3(unsigned(grid), 8 * NT), dim3(128), k_paged_join<__nv_bfloat16, 32 * DC>, p, 8 * NT);
 }
 
@@ -152,6 +150,8 @@ void decode(const PagedArgs& a, const chroma_b200_attention& g, int storage, cud
     want(items < kMaxRows, "more than 2^30 heads");
     p.least = 16;
     const int64_t size = int64_t(element(storage));
+    p.full = a.dim == space.pad;
+    p.kp = a.kp * size, p.kr = a.kr * size, p.vp = a.vp * size, p.vr = a.vr * size;
     p.q_vector = aligned16(a.q) && a.qt * size % 16 == 0 && a.qh * size % 16 == 0;
     if (!p.whole) {
         want(g.workspace && g.workspace_bytes >= space.bytes, "workspace too small");

@@ -22,6 +22,8 @@ struct PagedDecodeArgs {
     int whole;       // one CTA per item, no cuts
     int least;       // no cut leaves a CTA fewer units than this
     int q_vector;    // query rows are 16-byte aligned
+    int full;        // head rows fill the padded row
+    int64_t kp, kr, vp, vr;  // bytes between pages, rows
     float* parts;    // [2 * CTAs][heads of a block][padded dim]
     float2* part_ml; // [2 * CTAs][heads of a block]: maximum (log2 domain) and sum
     int4* joins;     // [CTAs]: slot, item of the slot, CTAs after this one, first part's number
@@ -131,9 +133,14 @@ __device__ __forceinline__ CtaPart<U> cut_line(const PagedDecodeArgs& p, int ite
     return part;
 }
 
-__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool ok) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(ok ? 16 : 0)
-                 : "memory");
+// 16 bytes of a cache row, read once: past L1. In the order written, so that they are under way before what follows.
+__device__ __forceinline__ uint4 load_word(const char* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint4 load_word_if(const char* p, bool ok) {
+    return ok ? load_word(p) : make_uint4(0, 0, 0, 0);
 }
 __device__ __forceinline__ float exp2_sfu(float x) {  // 2^-inf = 0
     float y;
@@ -173,13 +180,6 @@ __device__ __forceinline__ HeadEnd head_end(float m, float l, float sink) {
     return HeadEnd{c, sum == 0.f ? 0.f : 1.f / sum, sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2};
 }
 
-// Shared memory of k_paged_decode: each warp's ring of stages, then the merge buffer [8 warps][8 heads][32 DC].
-template <int DC> struct DecodeShape {
-    static constexpr int kStages = DC == 1 ? 4 : 3;
-    static constexpr int kStage = DC * 2 * 512 + (DC + 1) / 2 * 4 * 512;  // 16 positions of K, of V
-    static constexpr int kSmem = kDecWarps * (kStages * kStage + 8 * 32 * DC * 4);
-};
-
 // bf16, U = 16 positions per unit, head rows of up to 32 DC values, NT tiles of 8 query heads.
 //
 // Scores as S^T = K Q^T with mma.m16n8k16 (16 keys x 8 heads), outputs as O^T += V^T P^T (16 dims x 8 heads): the 8
@@ -196,116 +196,124 @@ template <int DC> struct DecodeShape {
 template <int DC, int NT, bool kAligned>
 __global__ void __launch_bounds__(kDecThreads, DC == 4 ? 1 : 2) k_paged_decode(PagedDecodeArgs p) {
     constexpr int U = 16, DB = (DC + 1) / 2, DP = 32 * DC;
-    constexpr int kStages = DecodeShape<DC>::kStages, kStage = DecodeShape<DC>::kStage;
-    extern __shared__ __align__(16) uint8_t dec_smem[];
+    __shared__ __align__(16) float merge[kDecWarps * 8 * DP];
     __shared__ float2 warp_ml[kDecWarps][8];
     const PagedArgs& a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    uint8_t* ring = dec_smem + warp * kStages * kStage + lane * 16;
-    float* merge = reinterpret_cast<float*>(dec_smem + kDecWarps * kStages * kStage);
     const int items = a.kv * p.blocks;
     asm volatile("griddepcontrol.launch_dependents;" :::);
 
     UnitCursor<U> at;
     const CtaPart<U> part = cut_line<U>(p, items, at);
     int4 join = make_int4(0, 0, 0, 0);
-    if (part.count == 0) {
+    const int count = int(part.count);
+    if (count == 0) {
         if (!p.whole && threadIdx.x == 0) p.joins[blockIdx.x] = join;
         return;
     }
 
-    // ---- issue side: this warp's units in turn, kStages - 1 ahead
+    // ---- load side: this warp's units in turn, one ahead
     UnitCursor<U> next = at;
-    int64_t next_index = warp;
+    int next_index = warp, next_id = -1, next_row = 0;
     next.u += warp;
     next.normalise(a, items);
-    int next_id = -1;
-    const auto page_of = [&](int j) {  // page of position j of the next unit's slot, or -1
+    // Byte addresses of this lane's share of row 0 of page 0 for the item's key-value head, and its other rows.
+    const char *klane, *vlane;
+    const int64_t k8 = a.kr * 16, v1 = a.vr * 2, v8 = a.vr * 16;
+    const auto enter_item = [&] {
+        const int64_t kvh = next.item / p.blocks;
+        klane = static_cast<const char*>(a.k) + (kvh * a.kh + g * a.kr + t * 8) * 2;
+        vlane = static_cast<const char*>(a.v) + (kvh * a.vh + 2 * t * a.vr + g * 8) * 2;
+    };
+    const auto page_of = [&](int j, int& row) {  // page of position j of the next unit's slot (or -1), and its row
         const int entry = int(a.by_page.div(uint32_t(j)));
+        row = j - entry * a.page;
         if (entry >= a.width) return -1;
         const int id = __ldg(a.table + next.slot * a.ts + entry);
         return id < a.pages ? id : -1;
     };
-    const auto fetch_id = [&] {
-        if (kAligned && next_index < part.count) next_id = page_of(next.seen.begin(next.u));
+    const auto fetch_id = [&] {  // a unit ahead of its use
+        if (kAligned) next_id = page_of(next.seen.begin(next.u), next_row);
     };
-    fetch_id();
-    const auto* kpool = static_cast<const __nv_bfloat16*>(a.k);
-    const auto* vpool = static_cast<const __nv_bfloat16*>(a.v);
-    uint32_t flags = 0;  // visibility of this lane's two keys, two bits per stage in flight, the last one lowest
-    const auto issue = [&](int stage) {
-        flags <<= 2;
-        if (next_index < part.count) {
-            const int j0 = next.seen.begin(next.u), pos = next.seen.pos;
-            const int64_t kvh = next.item / p.blocks;
-            uint8_t* dst = ring + stage * kStage;
-            uint32_t seen = 0;
-            if (kAligned) {
-                const int row = j0 - int(a.by_page.div(uint32_t(j0))) * a.page;
-                const bool here = next_id >= 0;
-                const int64_t id = here ? next_id : 0;
-                const bool all = j0 + U - 1 <= pos && (a.window <= 0 || pos - j0 < a.window || j0 + U <= a.first);
-                const auto* k = kpool + id * a.kp + kvh * a.kh + (row + g) * a.kr + t * 8;
-                const auto* v = vpool + id * a.vp + kvh * a.vh + (row + 2 * t) * a.vr + g * 8;
+    if (next_index < count) {
+        enter_item();
+        fetch_id();
+    }
+    uint4 kw[DC][2], vw[DB][4];  // the next unit's words of K (chunk, key g or g + 8) and V (64 dims, key)
+    int next_flags = 0;          // visibility of this lane's two keys
+    bool fast = false;           // every row, every word
+    const auto load_keys = [&] {
+        next_flags = 0;
+        if (next_index >= count) return;
+        const int j0 = next.seen.begin(next.u), pos = next.seen.pos;
+        const bool all = j0 + U - 1 <= pos && (a.window <= 0 || pos - j0 < a.window || j0 + U <= a.first);
+        fast = kAligned && all && next_id >= 0 && p.full;
+        if (fast) {
+            const char* k = klane + p.kp * next_id + p.kr * next_row;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const bool ok = here && (all || sees(pos, j0 + g + 8 * h, a.window, a.first));
-                    seen |= uint32_t(ok) << h;
-#pragma unroll
-                    for (int c = 0; c < DC; ++c)
-                        cp_async16_or_zero(dst + (c * 2 + h) * 512, k + h * 8 * a.kr + c * 32, ok && c * 32 + t * 8 < a.dim);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = (e & 1) + (e >> 1) * 8;
-                    const bool ok = here && (all || sees(pos, j0 + 2 * t + r, a.window, a.first));
-#pragma unroll
-                    for (int d = 0; d < DB; ++d)
-                        cp_async16_or_zero(dst + (DC * 2 + d * 4 + e) * 512, v + r * a.vr + d * 64, ok && d * 64 + g * 8 < a.dim);
-                }
-            } else {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int j = j0 + g + 8 * h, id = page_of(j), row = j - int(a.by_page.div(uint32_t(j))) * a.page;
-                    const bool ok = id >= 0 && sees(pos, j, a.window, a.first);
-                    seen |= uint32_t(ok) << h;
-                    const auto* k = kpool + (ok ? id * a.kp + row * a.kr + kvh * a.kh + t * 8 : 0);
-#pragma unroll
-                    for (int c = 0; c < DC; ++c) cp_async16_or_zero(dst + (c * 2 + h) * 512, k + c * 32, ok && c * 32 + t * 8 < a.dim);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = j0 + 2 * t + (e & 1) + (e >> 1) * 8, id = page_of(j);
-                    const int row = j - int(a.by_page.div(uint32_t(j))) * a.page;
-                    const bool ok = id >= 0 && sees(pos, j, a.window, a.first);
-                    const auto* v = vpool + (ok ? id * a.vp + row * a.vr + kvh * a.vh + g * 8 : 0);
-#pragma unroll
-                    for (int d = 0; d < DB; ++d)
-                        cp_async16_or_zero(dst + (DC * 2 + d * 4 + e) * 512, v + d * 64, ok && d * 64 + g * 8 < a.dim);
-                }
+            for (int c = 0; c < DC; ++c) {
+                kw[c][0] = load_word(k + c * 64);
+                kw[c][1] = load_word(k + k8 + c * 64);
             }
-            flags |= seen;
-            next_index += kDecWarps;
-            next.u += kDecWarps;
-            if (next_index < part.count) {
-                next.normalise(a, items);
-                fetch_id();
+            next_flags = 3;
+        } else {  // rows that are not seen, and words past the head's row, are zeros
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int j = j0 + g + 8 * h;
+                int row = next_row + 8 * h, id = next_id;
+                if (!kAligned) id = page_of(j, row), row -= g;
+                const bool ok = id >= 0 && (all || sees(pos, j, a.window, a.first));
+                next_flags |= int(ok) << h;
+                const char* k = klane + p.kp * id + p.kr * row;
+#pragma unroll
+                for (int c = 0; c < DC; ++c) kw[c][h] = load_word_if(k + c * 64, ok && c * 32 + t * 8 < a.dim);
             }
         }
-        cp_async_commit();
     };
-    int fill = 0, use = 0;
+    // The values of the unit whose keys were loaded last; then the cursor moves on.
+    const auto load_values = [&] {
+        if (next_index >= count) return;
+        if (fast) {
+            const char* v = vlane + p.vp * next_id + p.vr * next_row;
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) issue(s);
-    fill = kStages - 1;
+            for (int d = 0; d < DB; ++d) {
+                vw[d][0] = load_word(v + d * 128);
+                vw[d][1] = load_word(v + v1 + d * 128);
+                vw[d][2] = load_word(v + v8 + d * 128);
+                vw[d][3] = load_word(v + v8 + v1 + d * 128);
+            }
+        } else {
+            const int j0 = next.seen.begin(next.u), pos = next.seen.pos;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = (e & 1) + (e >> 1) * 8, j = j0 + 2 * t + r;
+                int row = next_row + r, id = next_id;
+                if (!kAligned) id = page_of(j, row), row -= 2 * t;
+                const bool ok = id >= 0 && sees(pos, j, a.window, a.first);
+                const char* v = vlane + p.vp * id + p.vr * row;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) vw[d][e] = load_word_if(v + d * 128, ok && d * 64 + g * 8 < a.dim);
+            }
+        }
+        next_index += kDecWarps;
+        next.u += kDecWarps;
+        if (next_index < count) {
+            if (next.u >= next.seen.units) {
+                next.normalise(a, items);
+                enter_item();
+            }
+            fetch_id();
+        }
+    };
+    load_keys();
+    load_values();
 
     // ---- use side, item by item
-    int64_t done = 0;
+    int done = 0;
     int slot = at.slot, item = at.item, u0 = at.u;
     SeenUnits<U> seen = at.seen;
-    while (done < part.count) {
-        const int64_t left = part.count - done;
-        const int take = int(left < seen.units - u0 ? left : seen.units - u0);
+    while (done < count) {
+        const int take = min(count - done, seen.units - u0);
         const int kvh = item / p.blocks, head0 = (item % p.blocks) * 8 * NT;  // within the group
         uint4 q[NT][DC];
 #pragma unroll
@@ -334,35 +342,30 @@ __global__ void __launch_bounds__(kDecThreads, DC == 4 ? 1 : 2) k_paged_decode(P
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[n][j][e] = 0.f;
         }
-        const int64_t end = done + take;
-        for (int64_t k = done + ((warp - int(done % kDecWarps) + kDecWarps) % kDecWarps); k < end; k += kDecWarps) {
-            issue(fill);
-            fill = fill + 1 == kStages ? 0 : fill + 1;
-            cp_async_wait<kStages - 1>();
-            const uint8_t* src = ring + use * kStage;
-            const uint32_t vis = flags >> (2 * (kStages - 1));
-            use = use + 1 == kStages ? 0 : use + 1;
-            float s[NT][4];
+        const int end = done + take;
+        for (int k = done + (unsigned(warp - done) % kDecWarps); k < end; k += kDecWarps) {
+            const int vis = next_flags;
+            float s[NT][4], half[NT][4];  // two chains of products
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+                for (int e = 0; e < 4; ++e) s[n][e] = half[n][e] = 0.f;
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
-                const uint4 ka = *reinterpret_cast<const uint4*>(src + (c * 2) * 512);
-                const uint4 kb = *reinterpret_cast<const uint4*>(src + (c * 2 + 1) * 512);
+                const uint4 ka = kw[c][0], kb = kw[c][1];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     mma_16816(s[n], ka.x, kb.x, ka.y, kb.y, q[n][c].x, q[n][c].y);
-                    mma_16816(s[n], ka.z, kb.z, ka.w, kb.w, q[n][c].z, q[n][c].w);
+                    mma_16816(half[n], ka.z, kb.z, ka.w, kb.w, q[n][c].z, q[n][c].w);
                 }
             }
+            load_keys();
             bool grow = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[n][e] *= a.scale_log2;
+                    s[n][e] = (s[n][e] + half[n][e]) * a.scale_log2;
                     if (!((vis >> (e >> 1)) & 1)) s[n][e] = -INFINITY;
                 }
                 grow |= fmaxf(s[n][0], s[n][2]) > m[n][0] + 8.f || fmaxf(s[n][1], s[n][3]) > m[n][1] + 8.f;
@@ -399,9 +402,7 @@ __global__ void __launch_bounds__(kDecThreads, DC == 4 ? 1 : 2) k_paged_decode(P
             }
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                uint4 v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const uint4*>(src + (DC * 2 + d * 4 + e) * 512);
+                const auto& v = vw[d];
                 const auto word = [](const uint4& x, int j) { return j == 0 ? x.x : j == 1 ? x.y : j == 2 ? x.z : x.w; };
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {  // dims 64 d + 8 g + 2 j (rows g) and + 1 (rows g + 8)
@@ -413,6 +414,7 @@ __global__ void __launch_bounds__(kDecThreads, DC == 4 ? 1 : 2) k_paged_decode(P
                     for (int n = 0; n < NT; ++n) mma_16816(o[n][d * 4 + j], a0, a1, a2, a3, pb[n][0], pb[n][1]);
                 }
             }
+            load_values();
         }
         // ---- the item's end: merge the warps, then finish it or leave its part
         const bool complete = u0 == 0 && take == seen.units;
