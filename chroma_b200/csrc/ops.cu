@@ -2,6 +2,8 @@
 // their arguments, choice of kernel, launches. Nothing here allocates or synchronises.
 #include "../../include/chroma_b200.h"
 
+#include <cuda.h>
+
 #include <cstdio>
 #include <stdexcept>
 #include <string>
@@ -118,37 +120,97 @@ PoolArgs pool_args(const chroma_b200_pages& p) {
     return a;
 }
 
-// Workspace of a decode: partial results of two items per CTA, and each CTA's join.
+// Timeouts of bounded waits on this device, read by chroma_b200_operators_check.
+__device__ unsigned g_error;
+
+unsigned* error_word() {
+    void* at = nullptr;
+    check(cudaGetSymbolAddress(&at, g_error), "error word");
+    return static_cast<unsigned*>(at);
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// Boxes of 64 values, one head, `rows` rows of one page of a bf16 pool, 128-byte swizzle. False where the pool's strides
+// are none that the TMA engine takes.
+bool page_map(CUtensorMap* map, const void* pool, const PagedArgs& a, int64_t kp, int64_t kr, int64_t kh, int rows) {
+    static const EncodeTiled encode = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        check(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q), "cuTensorMapEncodeTiled");
+        if (!p || q != cudaDriverEntryPointSuccess) throw std::runtime_error("cuTensorMapEncodeTiled unavailable");
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    const cuuint64_t dims[4] = {cuuint64_t(a.dim), cuuint64_t(a.kv), cuuint64_t(a.page), cuuint64_t(a.pages)};
+    const cuuint64_t strides[3] = {cuuint64_t(kh * 2), cuuint64_t(kr * 2), cuuint64_t(kp * 2)};
+    const cuuint32_t box[4] = {64, 1, cuuint32_t(rows), 1}, step[4] = {1, 1, 1, 1};
+    for (const cuuint64_t s : strides)
+        if (s == 0 || s >> 40) return false;
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(pool), dims, strides, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// How a decode is laid out, and its workspace: partial results of two items per CTA, and each CTA's join.
 struct DecodeSpace {
-    int grid, tiles, pad;  // CTAs, tiles of 8 heads in a block, padded head row
+    int grid, tiles, pad, blocks;  // CTAs at most, tiles of 8 heads in an item, padded head row, items per kv head
     int64_t parts, ml, bytes;
     DecodeSpace(int heads, int kv, int dim) {
         const int group = heads / kv;
         tiles = group > 8 ? 2 : 1;
         pad = dim <= 32 ? 32 : dim <= 64 ? 64 : 128;
-        grid = sm_count() * (pad == 128 ? 1 : 2);
-        parts = int64_t(2) * grid * 8 * tiles * pad * 4;
-        ml = int64_t(2) * grid * 8 * tiles * 8;
+        blocks = (group + 8 * tiles - 1) / (8 * tiles);
+        grid = sm_count() * 4;
+        const int64_t rows = int64_t(2) * grid * 8 * tiles;
+        parts = rows * pad * 4;
+        ml = rows * 8;
         bytes = parts + ml + int64_t(grid) * 16;
     }
 };
 
-template <int DC, int NT> void decode_bf16(const PagedDecodeArgs& p, int grid, bool aligned, cudaStream_t s) {
-    const auto kernel = aligned ? k_paged_decode<DC, NT, true> : k_paged_decode<DC, NT, false>;
-    launch(s, dim3(unsigned(grid)), dim3(kDecThreads), 0, kernel, p);
-    if (!p.whole) launch_after(s, dim3(unsigned(grid), 8 * NT), dim3(128), k_paged_join<__nv_bfloat16, 32 * DC>, p, 8 * NT);
+template <int DC, int NT> void decode_join(const PagedDecodeArgs& p, int grid, cudaStream_t s) {
+    if (p.whole) return;
+    // A warp joins few parts by itself; where a line has few sequences for its CTAs, their items have many parts.
+    const int line = grid / (p.a.kv * p.blocks);
+    if (p.a.slots >= line / 4) launch_after(s, dim3(unsigned(grid), NT), dim3(256), k_paged_join<__nv_bfloat16, 32 * DC, true>, p, 8 * NT);
+    else launch_after(s, dim3(unsigned(grid), 8 * NT), dim3(256), k_paged_join<__nv_bfloat16, 32 * DC, false>, p, 8 * NT);
+}
+
+template <int DC, int NT> void decode_bf16(PagedDecodeArgs& p, int64_t items, cudaStream_t s) {
+    const PagedArgs& a = p.a;
+    CUtensorMap kmap, vmap;
+    if constexpr (DC != 1) {
+        using Ring = DecodeRing<DC>;
+        p.box = a.page % Ring::U == 0 ? Ring::U : 16;
+        if (p.full && a.page % 16 == 0 && page_map(&kmap, a.k, a, a.kp, a.kr, a.kh, p.box) && page_map(&vmap, a.v, a, a.vp, a.vr, a.vh, p.box)) {
+            const int grid = p.whole ? int(items) : sm_count() * 2;
+            p.least = 2 * Ring::kWarps;
+            check(cudaFuncSetAttribute(k_paged_decode_tma<DC, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring::kSmem), "smem attribute");
+            launch(s, dim3(unsigned(grid)), dim3(32 * Ring::kWarps), Ring::kSmem, k_paged_decode_tma<DC, NT>, p, kmap, vmap);
+            return decode_join<DC, NT>(p, grid, s);
+        }
+    }
+    using Regs = DecodeRegs<DC, NT>;
+    const auto kernel = a.page % 16 == 0 ? k_paged_decode<DC, NT, true> : k_paged_decode<DC, NT, false>;
+    const int grid = p.whole ? int(items) : sm_count() * Regs::kCtas;
+    p.least = 2 * Regs::kWarps;
+    launch(s, dim3(unsigned(grid)), dim3(32 * Regs::kWarps), 0, kernel, p);
+    decode_join<DC, NT>(p, grid, s);
 }
 
 void decode(const PagedArgs& a, const chroma_b200_attention& g, int storage, cudaStream_t s) {
     const DecodeSpace space(a.heads, a.kv, a.dim);
     PagedDecodeArgs p{};
     p.a = a;
-    p.blocks = (a.group + 8 * space.tiles - 1) / (8 * space.tiles);
-    const int64_t items = int64_t(a.slots) * a.kv * p.blocks;
-    // Short tables need no cut: at 1,024 positions an item is 8 units a warp. Neither do many items: they even out.
-    p.whole = int64_t(a.width) * a.page <= 1024 || items >= int64_t(16) * space.grid;
+    p.blocks = space.blocks;
+    p.error = error_word();
+    const int64_t lines = int64_t(a.kv) * p.blocks, items = a.slots * lines;
     want(items < kMaxRows, "more than 2^30 heads");
-    p.least = 16;
+    // One CTA per item where a warp has at most four units of 16 anyway, where there are so many items that they even
+    // out, and where the heads alone outnumber the CTAs.
+    p.whole = int64_t(a.width) * a.page <= 256 || items >= int64_t(8) * space.grid || lines > sm_count();
     const int64_t size = int64_t(element(storage));
     p.full = a.dim == space.pad;
     p.kp = a.kp * size, p.kr = a.kr * size, p.vp = a.vp * size, p.vr = a.vr * size;
@@ -159,11 +221,9 @@ void decode(const PagedArgs& a, const chroma_b200_attention& g, int storage, cud
         p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(g.workspace) + space.parts);
         p.joins = reinterpret_cast<int4*>(static_cast<char*>(g.workspace) + space.parts + space.ml);
     }
-    const int grid = p.whole ? int(items) : space.grid;
-    const bool aligned = a.page % 16 == 0;
     const auto by_dim = [&](auto dc) {
-        if (space.tiles == 2) decode_bf16<decltype(dc)::value, 2>(p, grid, aligned, s);
-        else decode_bf16<decltype(dc)::value, 1>(p, grid, aligned, s);
+        if (space.tiles == 2) decode_bf16<decltype(dc)::value, 2>(p, items, s);
+        else decode_bf16<decltype(dc)::value, 1>(p, items, s);
     };
     if (space.pad == 32) by_dim(std::integral_constant<int, 1>());
     else if (space.pad == 64) by_dim(std::integral_constant<int, 2>());
