@@ -13,6 +13,7 @@
 #include "logits.cuh"
 #include "paged.cuh"
 #include "paged_decode.cuh"
+#include "paged_prompt.cuh"
 #include "pages.cuh"
 
 namespace {
@@ -230,6 +231,32 @@ void decode(const PagedArgs& a, const chroma_b200_attention& g, int storage, cud
     else by_dim(std::integral_constant<int, 4>());
 }
 
+template <int H> void prompt_bf16(PagedPromptArgs& p, cudaStream_t s) {
+    const PagedArgs& a = p.a;
+    CUtensorMap kmap{}, vmap{};
+    p.box = 0;
+    for (int rows = kPrTile; rows >= 8 && !p.box; rows /= 2)
+        if (a.page % rows == 0) p.box = rows;
+    if (p.box && !(page_map(&kmap, a.k, a, a.kp, a.kr, a.kh, p.box) && page_map(&vmap, a.v, a, a.vp, a.vr, a.vh, p.box))) p.box = 0;
+    const int64_t tiles = int64_t(a.tokens) * a.group / 256 + a.slots;  // at least as many as there are
+    const int64_t items = tiles * a.kv;
+    const int grid = int(items < sm_count() ? items : sm_count());
+    check(cudaFuncSetAttribute(k_paged_prompt<H>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<H>::kSmem), "smem attribute");
+    launch(s, dim3(unsigned(grid)), dim3(kPrThreads), PromptShape<H>::kSmem, k_paged_prompt<H>, p, kmap, vmap);
+}
+
+void prompt(const PagedArgs& a, int storage, cudaStream_t s) {
+    PagedPromptArgs p{};
+    p.a = a;
+    p.by_group = FastDiv(uint32_t(a.group));
+    p.error = error_word();
+    const int64_t size = int64_t(element(storage));
+    p.q_vector = aligned16(a.q) && a.qt * size % 16 == 0 && a.qh * size % 16 == 0;
+    p.out_vector = aligned16(a.out) && a.ot * size % 16 == 0 && a.oh * size % 16 == 0;
+    if (a.dim <= 64) prompt_bf16<1>(p, s);
+    else prompt_bf16<2>(p, s);
+}
+
 dim3 table_grid(const chroma_b200_pages& p) { return dim3(unsigned((p.width + 255) / 256), unsigned(p.slots)); }
 
 }  // namespace
@@ -277,6 +304,7 @@ int chroma_b200_paged_attention(const chroma_b200_pages* p, const chroma_b200_at
         want(g->heads > 0 && g->heads % p->kv_heads == 0, "heads must be a multiple of kv_heads");
         want(g->starts || g->tokens == p->slots, "without starts there is one token per slot");
         want(g->first >= 0, "first must be nonnegative");
+        want(g->scale > 0, "scale must be positive");
         want(int64_t(g->tokens) * g->heads <= kMaxRows, "more than 2^30 rows of queries");
         if (!g->tokens) return;
         want(g->q && g->out, "null argument");
@@ -293,6 +321,7 @@ int chroma_b200_paged_attention(const chroma_b200_pages* p, const chroma_b200_at
         a.window = g->window, a.first = g->first, a.scale_log2 = g->scale * kLog2e;
         const int64_t rows = int64_t(g->tokens) * g->heads;
         if (!g->starts && p->storage == CHROMA_B200_BF16) return decode(a, *g, p->storage, cudaStream_t(stream));
+        if (p->storage == CHROMA_B200_BF16) return prompt(a, p->storage, cudaStream_t(stream));
         by_type(p->storage, [&](auto t) {
             launch(cudaStream_t(stream), dim3(unsigned((rows + 3) / 4)), dim3(128), size_t(16) * p->head_dim,
                    k_paged_attention_rows<decltype(t)>, a);

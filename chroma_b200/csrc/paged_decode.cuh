@@ -12,6 +12,7 @@
 // k_paged_join needs no flags or counters.
 #pragma once
 
+#include "mma.cuh"
 #include "paged.cuh"
 #include "tcgen05.cuh"
 
@@ -129,41 +130,24 @@ __device__ __forceinline__ uint4 load_word(const char* p) {
 __device__ __forceinline__ uint4 load_word_if(const char* p, bool ok) {
     return ok ? load_word(p) : make_uint4(0, 0, 0, 0);
 }
-__device__ __forceinline__ float exp2_sfu(float x) {  // 2^-inf = 0
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// D (16 x 8, fp32) += A (16 x 16) B (16 x 8), bf16.
-__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                          uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
 
 // What is merged of one head over the warps of a CTA, over the parts of an item: weights 2^(m - M), where a part
 // without a finite maximum counts only if its sum does (NaN).
 __device__ __forceinline__ float part_weight(float m, float l, float top) {
-    return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2_sfu(m - top);
+    return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : fast_exp2(m - top);
 }
 
 // Final step of one head's element: o / (l + sink).
 struct HeadEnd { float c, inv, lse; };
 __device__ __forceinline__ HeadEnd head_end(float m, float l, float sink) {
     const float top = fmaxf(m, sink);
-    const float c = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2_sfu(m - top);
-    const float sum = l * c + (sink == -INFINITY ? 0.f : exp2_sfu(sink - top));
+    const float c = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : fast_exp2(m - top);
+    const float sum = l * c + (sink == -INFINITY ? 0.f : fast_exp2(sink - top));
     return HeadEnd{c, sum == 0.f ? 0.f : 1.f / sum, sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2};
 }
 
@@ -201,7 +185,7 @@ template <int NT, int MT> struct WarpState {
                     for (int kt = 0; kt < KT; ++kt) x = fmaxf(x, fmaxf(s[kt][n][e], s[kt][n][e + 2]));
                     for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
                     const float top = fmaxf(m[n][e], x);
-                    const float corr = m[n][e] == -INFINITY ? (l[n][e] == 0.f ? 0.f : 1.f) : exp2_sfu(m[n][e] - top);
+                    const float corr = m[n][e] == -INFINITY ? (l[n][e] == 0.f ? 0.f : 1.f) : fast_exp2(m[n][e] - top);
                     m[n][e] = top;
                     l[n][e] *= corr;
 #pragma unroll
@@ -216,13 +200,13 @@ template <int NT, int MT> struct WarpState {
             const float r0 = m[n][0] == -INFINITY ? 0.f : m[n][0], r1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
-                const float p0 = exp2_sfu(s[kt][n][0] - r0), p1 = exp2_sfu(s[kt][n][1] - r1);
-                const float p2 = exp2_sfu(s[kt][n][2] - r0), p3 = exp2_sfu(s[kt][n][3] - r1);
+                const float p0 = fast_exp2(s[kt][n][0] - r0), p1 = fast_exp2(s[kt][n][1] - r1);
+                const float p2 = fast_exp2(s[kt][n][2] - r0), p3 = fast_exp2(s[kt][n][3] - r1);
                 l[n][0] += p0 + p2;
                 l[n][1] += p1 + p3;
                 // The weights go into the product with 8 bits, as bf16 operands have; their sum keeps all of them.
-                pb[kt][n][0] = transpose_8x8(bf16_pair(p0, p1));
-                pb[kt][n][1] = transpose_8x8(bf16_pair(p2, p3));
+                pb[kt][n][0] = transpose_8x8(pack_bf16(p0, p1));
+                pb[kt][n][1] = transpose_8x8(pack_bf16(p2, p3));
             }
         }
     }
@@ -453,10 +437,11 @@ k_paged_decode(PagedDecodeArgs p) {
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
                 const uint4 ka = kw[c][0], kb = kw[c][1];
+                const uint32_t a0[4] = {ka.x, kb.x, ka.y, kb.y}, a1[4] = {ka.z, kb.z, ka.w, kb.w};
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    mma_16816(s[0][n], ka.x, kb.x, ka.y, kb.y, q[n][c].x, q[n][c].y);
-                    mma_16816(half[n], ka.z, kb.z, ka.w, kb.w, q[n][c].z, q[n][c].w);
+                    mma_bf16(s[0][n], a0, q[n][c].x, q[n][c].y);
+                    mma_bf16(half[n], a1, q[n][c].z, q[n][c].w);
                 }
             }
             load_keys();
@@ -473,12 +458,10 @@ k_paged_decode(PagedDecodeArgs p) {
                 const auto word = [](const uint4& x, int j) { return j == 0 ? x.x : j == 1 ? x.y : j == 2 ? x.z : x.w; };
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {  // dims 64 d + 8 g + 2 j (rows g) and + 1 (rows g + 8)
-                    const uint32_t a0 = __byte_perm(word(v[0], j), word(v[1], j), 0x5410);
-                    const uint32_t a1 = __byte_perm(word(v[0], j), word(v[1], j), 0x7632);
-                    const uint32_t a2 = __byte_perm(word(v[2], j), word(v[3], j), 0x5410);
-                    const uint32_t a3 = __byte_perm(word(v[2], j), word(v[3], j), 0x7632);
+                    const uint32_t f[4] = {__byte_perm(word(v[0], j), word(v[1], j), 0x5410), __byte_perm(word(v[0], j), word(v[1], j), 0x7632),
+                                           __byte_perm(word(v[2], j), word(v[3], j), 0x5410), __byte_perm(word(v[2], j), word(v[3], j), 0x7632)};
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_16816(w.o[n][d * 4 + j], a0, a1, a2, a3, pb[0][n][0], pb[0][n][1]);
+                    for (int n = 0; n < NT; ++n) mma_bf16(w.o[n][d * 4 + j], f, pb[0][n][0], pb[0][n][1]);
                 }
             }
             load_values();
@@ -499,14 +482,6 @@ template <int DC> struct DecodeRing {
     static constexpr int kSmem = 1024 + kWarps * (kStages * kStage + 8 * kMergeDims * 4);
 };
 
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
 // Box {64 values, 1 head, rows, 1 page} of a pool.
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, int d, int head, int row, int page,
                                               uint64_t* bar) {
@@ -629,9 +604,9 @@ k_paged_decode_tma(PagedDecodeArgs p, const __grid_constant__ CUtensorMap kmap, 
 #pragma unroll
                 for (int c = 0; c < MT; ++c) {
                     uint32_t f[4];
-                    ldmatrix4(f, ks + (c >> 2) * kHalf + (kt * 16 + krow) * 128 + ((((c & 3) * 2 + kcol) ^ (krow & 7)) << 4));
+                    ldsm_x4(f, ks + (c >> 2) * kHalf + (kt * 16 + krow) * 128 + ((((c & 3) * 2 + kcol) ^ (krow & 7)) << 4));
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_16816(c & 1 ? half[n] : s[kt][n], f[0], f[1], f[2], f[3], q[n][c][0], q[n][c][1]);
+                    for (int n = 0; n < NT; ++n) mma_bf16(c & 1 ? half[n] : s[kt][n], f, q[n][c][0], q[n][c][1]);
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -661,9 +636,9 @@ k_paged_decode_tma(PagedDecodeArgs p, const __grid_constant__ CUtensorMap kmap, 
 #pragma unroll
                 for (int c = 0; c < MT; ++c) {
                     uint32_t f[4];
-                    ldmatrix4_trans(f, vs + (c >> 2) * kHalf + (kt * 16 + vrow) * 128 + ((((c & 3) * 2 + vcol) ^ (vrow & 7)) << 4));
+                    ldsm_x4_t(f, vs + (c >> 2) * kHalf + (kt * 16 + vrow) * 128 + ((((c & 3) * 2 + vcol) ^ (vrow & 7)) << 4));
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_16816(w.o[n][c], f[0], f[1], f[2], f[3], pb[kt][n][0], pb[kt][n][1]);
+                    for (int n = 0; n < NT; ++n) mma_bf16(w.o[n][c], f, pb[kt][n][0], pb[kt][n][1]);
                 }
             __syncwarp();
             if (alive) issue();

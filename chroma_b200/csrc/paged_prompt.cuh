@@ -1,0 +1,527 @@
+// Attention of prompts over a paged cache on the 5th-generation tensor cores (bf16): chunks of any lengths, each after
+// what its sequence's pages hold already, causal, with a sliding window that keeps the first positions in sight.
+//
+// A row is one query head of one token; the rows of a key-value head are packed, token after token with its `group`
+// query heads side by side, so that a tile of 128 rows shares every key even where a chunk has few tokens. A work item
+// is 256 consecutive rows (two tiles) of one key-value head of one sequence, against key tiles of 128 positions. The
+// grid is persistent, one CTA per SM; items are taken from the last rows of the last sequence backwards (the most keys
+// first), the key-value heads of the same rows side by side. 11 warps:
+//   warps 0-3, 4-7  the online softmax of tile 0, 1, one row per thread (TMEM lane = row): the row of S (128 columns)
+//                   from TMEM at once, P = 2^(s - m) back over its first 64 columns as bf16 pairs; at the item's end
+//                   O / l to global memory
+//   warp 8          one thread issues, per key tile t and tile k in turn: O_k += P_k(t) V(t), S_k(t+1) = Q_k K(t+1)^T
+//   warp 9          K and V tiles into a ring, by TMA boxes of as many rows as divide the page (a box never leaves its
+//                   page), or, where the pool or the page size is none that TMA takes, row by row with cp.async
+//   warp 10         Q tiles of the next item, as soon as the last S of this one is done
+// P stays in tensor memory as the A operand of the product with V. The tensor core runs the products of one issuing
+// thread in order, so S_k(t+1) lands over P_k(t) only after O_k has taken it, and the commit that signals S_k(t+1)
+// covers that product too: the softmax may rescale O_k as soon as it sees S_k(t+1). The maximum moves only when a tile
+// exceeds it by more than 2^8, so O is rescaled rarely.
+//
+// A position that no row may see costs nothing (whole tiles are passed over) or a mask of 128 bits per row, applied only
+// to the tiles that need it. Values behind the end of a sequence are cleared in shared memory, since what lies there may
+// not be finite. Positions that some rows of a tile see and others do not meet the others with weight 0, which is no
+// protection against infinities: a row whose result is not finite is computed again, key by key.
+//
+// All waits are bounded (tma.cuh).
+#pragma once
+
+#include "mma.cuh"
+#include "paged.cuh"
+#include "tcgen05.cuh"
+
+namespace cb200 {
+
+constexpr int kPrThreads = 352, kPrTile = 128;
+
+struct PagedPromptArgs {
+    PagedArgs a;
+    FastDiv by_group;
+    int box;                 // rows of a TMA box; 0: row by row
+    int q_vector, out_vector;  // rows are 16-byte aligned
+    unsigned* error;
+};
+
+// 64 H values per row (H = 1, 2): Q tiles, then a ring of K and V tiles, in blocks of [128 rows][64 values] with the
+// 128-byte swizzle; then each stage's missing positions.
+template <int H> struct PromptShape {
+    static constexpr int kBlock = kPrTile * 128, kTile = H * kBlock, kStage = 2 * kTile, kStages = H == 2 ? 2 : 4;
+    static constexpr int kSmem = 1024 + 2 * kTile + kStages * kStage + kStages * 16;
+};
+
+// A work item: 256 rows of one key-value head of one slot, and the key tiles that they see.
+struct PromptItem {
+    int slot, kvh, row0, rows, token0, pos0;  // first row; rows of the slot; first token; its position
+    int tiles, pre, main0;                    // key tiles [0, pre), then from main0 on
+    int active;                               // tiles of rows: 1 or 2
+    __device__ __forceinline__ int key0(int t) const { return (t < pre ? t : main0 + t - pre) * kPrTile; }
+};
+
+// The items of a CTA in turn: blockIdx.x, + gridDim.x (backwards every other round, which evens out their sizes), ...
+struct PromptCursor {
+    int slot, before, round;  // tiles of the slots after `slot`
+    __device__ __forceinline__ explicit PromptCursor(const PagedArgs& a) : slot(a.slots - 1), before(0), round(0) {}
+    static __device__ __forceinline__ int rows_of(const PagedArgs& a, int s) {
+        const int t0 = min(max(a.starts[s], 0), a.tokens), t1 = min(max(a.starts[s + 1], 0), a.tokens);
+        return max(0, t1 - t0) * a.group;
+    }
+    __device__ __forceinline__ bool next(const PagedPromptArgs& p, int total, PromptItem& w) {
+        const PagedArgs& a = p.a;
+        const int64_t i = int64_t(round) * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        ++round;
+        if (i >= int64_t(total) * a.kv) return false;
+        const int tile = int(i / a.kv);
+        w.kvh = int(i % a.kv);
+        int rows = rows_of(a, slot), n = (rows + 255) / 256;
+        while (tile >= before + n) {
+            before += n;
+            --slot;
+            rows = rows_of(a, slot);
+            n = (rows + 255) / 256;
+        }
+        w.slot = slot;
+        w.rows = rows;
+        w.row0 = (n - 1 - (tile - before)) * 256;
+        w.token0 = min(max(a.starts[slot], 0), a.tokens);
+        w.pos0 = held_rows(a.lengths, slot, a.width, a.page) - rows / a.group;
+        w.active = w.row0 + kPrTile < rows ? 2 : 1;
+        const int first = w.pos0 + int(p.by_group.div(w.row0)), last = w.pos0 + int(p.by_group.div(min(w.row0 + 256, rows) - 1));
+        const int low = a.window > 0 ? max(0, first - a.window + 1) : 0;
+        w.pre = (min(a.first, low) + kPrTile - 1) / kPrTile;
+        w.main0 = max(low / kPrTile, w.pre);
+        w.tiles = last < 0 ? 0 : w.pre + max(0, last / kPrTile - w.main0 + 1);
+        return true;
+    }
+};
+
+// Softmax attention of one row, key by key, by one warp: any mask, any values. o[c] is dim 32 c + lane.
+template <typename T>
+__device__ __noinline__ void attend_row(const PagedArgs& a, int token, int head, int slot, int pos, float& m, float& l,
+                                        float (&o)[4]) {
+    const int lane = threadIdx.x & 31, kvh = head / a.group;
+    const T* q = static_cast<const T*>(a.q) + token * a.qt + head * a.qh;
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = 0.f;
+    const int low = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    const int first = min(a.first, low);  // [0, first) then [low, pos]
+    const int total = max(0, pos + 1 - low + first);
+    for (int base = 0; base < total; base += 32) {
+        const int i = base + lane;
+        const int j = i < first ? i : low + i - first;
+        const int entry = i < total ? int(a.by_page.div(uint32_t(j))) : 0;
+        int id = i < total ? a.table[slot * a.ts + entry] : -1;
+        if (id >= a.pages) id = -1;
+        float s = -INFINITY;
+        const int row = j - entry * a.page;
+        if (id >= 0) {
+            const T* k = static_cast<const T*>(a.k) + id * a.kp + row * a.kr + kvh * a.kh;
+            float dot = 0.f;
+            for (int d = 0; d < a.dim; ++d) dot = fmaf(Store<T>::load(q + d), Store<T>::load(k + d), dot);
+            s = dot * a.scale_log2;
+        }
+        const float mx = fmaxf(m, warp_max(s));
+        if (mx == -INFINITY && !__any_sync(0xffffffffu, isnan(s))) continue;
+        const float corr = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - mx);
+        const float p = id < 0 ? 0.f : exp2f(s - mx);
+        l = l * corr + warp_sum(p);
+        m = mx;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] *= corr;
+        for (int e = 0; e < min(32, total - base); ++e) {
+            const int ide = __shfl_sync(0xffffffffu, id, e), rowe = __shfl_sync(0xffffffffu, row, e);
+            const float pe = __shfl_sync(0xffffffffu, p, e);
+            if (ide < 0) continue;
+            const T* v = static_cast<const T*>(a.v) + ide * a.vp + rowe * a.vr + kvh * a.vh;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (c * 32 + lane < a.dim) o[c] = fmaf(pe, Store<T>::load(v + c * 32 + lane), o[c]);
+        }
+    }
+}
+
+// Writes what attend_row found.
+template <typename T>
+__device__ __forceinline__ void finish_row(const PagedArgs& a, int token, int head, float m, float l, const float (&o)[4]) {
+    const int lane = threadIdx.x & 31;
+    const float sink = sink_log2<T>(a.sinks, a.sinks_fp32, head);
+    const float top = fmaxf(m, sink);
+    const float c = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - top);
+    const float sum = l * c + (sink == -INFINITY ? 0.f : exp2f(sink - top));
+    T* orow = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e * 32 + lane < a.dim) Store<T>::store(orow + e * 32 + lane, sum == 0.f ? 0.f : o[e] * c / sum);
+    if (a.lse && lane == 0) a.lse[int64_t(token) * a.heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+__device__ __forceinline__ uint32_t bits_from_to(int lo, int hi) {  // bits lo..hi of a word, cut to it
+    lo = max(lo, 0);
+    hi = min(hi, 31);
+    return hi < lo ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
+}
+
+template <int H>
+__global__ void __launch_bounds__(kPrThreads, 1)
+k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    using Shape = PromptShape<H>;
+    constexpr int kStages = Shape::kStages, D = 64 * H;
+    extern __shared__ uint8_t pr_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pr_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* Qs = sm;                           // [2][H][128][64]
+    uint8_t* KV = Qs + 2 * Shape::kTile;        // stage s: K at s * kStage, V kTile behind it
+    uint32_t* gone = reinterpret_cast<uint32_t*>(KV + kStages * Shape::kStage);  // [kStages][4]
+    __shared__ uint64_t q_full[2], q_empty[2], kv_full[kStages], kv_empty[kStages], s_full[2], p_full[2], o_done[2];
+    __shared__ uint32_t tmem_base;
+    __shared__ int s_total;
+    __shared__ volatile int abort_flag;
+    const PagedArgs& a = p.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int k = 0; k < 2; ++k) {
+            mbar_init(&q_full[k], 1);
+            mbar_init(&q_empty[k], 1);
+            mbar_init(&s_full[k], 1);
+            mbar_init(&p_full[k], 4);
+            mbar_init(&o_done[k], 1);
+        }
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&kv_full[s], 1);
+            mbar_init(&kv_empty[s], 1);
+        }
+        abort_flag = 0;
+        s_total = 0;
+        fence_barrier_init();
+    }
+    if (warp == 8) {
+        tmem_alloc(&tmem_base, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    {
+        int mine = 0;
+        for (int s = threadIdx.x; s < a.slots; s += kPrThreads) mine += (PromptCursor::rows_of(a, s) + 255) / 256;
+        if (mine) atomicAdd(&s_total, mine);
+    }
+    __syncthreads();
+    const int total = s_total;
+    const uint32_t tmem = tmem_base;
+    PromptCursor cursor(a);
+    PromptItem w;
+
+    if (warp == 9) {
+        // ---- K and V
+        int g = 0;  // tiles so far
+        while (!abort_flag && cursor.next(p, total, w)) {
+            for (int t = 0; t < w.tiles; ++t, ++g) {
+                const int s = g % kStages;
+                if (!mbar_wait(&kv_empty[s], unsigned((g / kStages) & 1) ^ 1, p.error)) abort_flag = 1;
+                if (abort_flag) break;
+                const int j0 = w.key0(t);
+                uint8_t* kd = KV + s * Shape::kStage;
+                if (lane < 4) gone[s * 4 + lane] = 0;
+                __syncwarp();
+                if (p.box) {
+                    const int boxes = kPrTile / p.box;
+                    int row = 0, id = a.pages;  // beyond the map: zeros
+                    if (lane < boxes) {
+                        const int j = j0 + lane * p.box, entry = int(a.by_page.div(uint32_t(j)));
+                        row = j - entry * a.page;
+                        if (entry < a.width) id = __ldg(a.table + w.slot * a.ts + entry);
+                        if (id < 0 || id >= a.pages) {
+                            id = a.pages;
+                            for (int e = lane * p.box; e < (lane + 1) * p.box; e += 8)
+                                atomicOr(&gone[s * 4 + (e >> 5)], 0xffu << (e & 31));
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], Shape::kStage);
+                    __syncwarp();
+                    if (lane < boxes)
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            uint8_t* to = kd + h * Shape::kBlock + lane * p.box * 128;
+                            asm volatile(
+                                "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(to)),
+                                "l"(reinterpret_cast<uint64_t>(&kmap)), "r"(h * 64), "r"(w.kvh), "r"(row), "r"(id), "r"(smem_addr(&kv_full[s]))
+                                : "memory");
+                            asm volatile(
+                                "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(to + Shape::kTile)),
+                                "l"(reinterpret_cast<uint64_t>(&vmap)), "r"(h * 64), "r"(w.kvh), "r"(row), "r"(id), "r"(smem_addr(&kv_full[s]))
+                                : "memory");
+                        }
+                } else {
+                    const int end = held_rows(a.lengths, w.slot, a.width, a.page);
+                    for (int base = 0; base < kPrTile; base += 32) {  // a row per lane, its address handed round
+                        const int j = j0 + base + lane, entry = int(a.by_page.div(uint32_t(j)));
+                        int id = j < end ? __ldg(a.table + w.slot * a.ts + entry) : -1;
+                        if (id >= a.pages) id = -1;
+                        const int row = j - entry * a.page;
+                        const uint32_t none = __ballot_sync(0xffffffffu, id < 0);
+                        if (lane == 0) gone[s * 4 + (base >> 5)] = none;
+                        const int64_t ko = id < 0 ? 0 : id * a.kp + row * a.kr + w.kvh * a.kh;
+                        const int64_t vo = id < 0 ? 0 : id * a.vp + row * a.vr + w.kvh * a.vh;
+                        constexpr int kChunks = 8 * H, kRows = 32 / kChunks;  // 16-byte chunks of a row, rows at a time
+                        for (int r0 = 0; r0 < 32; r0 += kRows) {
+                            const int r = r0 + lane / kChunks, c = lane % kChunks;
+                            const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+                            const bool ok = !(none >> r & 1) && c * 8 < a.dim;
+                            uint8_t* to = kd + (c >> 3) * Shape::kBlock + (base + r) * 128 + (((c & 7) ^ (r & 7)) << 4);
+                            const auto* ks = static_cast<const __nv_bfloat16*>(a.k) + kr + (ok ? c * 8 : 0);
+                            const auto* vs = static_cast<const __nv_bfloat16*>(a.v) + vr + (ok ? c * 8 : 0);
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(to)), "l"(ks), "r"(ok ? 16 : 0) : "memory");
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(to + Shape::kTile)), "l"(vs), "r"(ok ? 16 : 0) : "memory");
+                        }
+                    }
+                    cp_async_commit();
+                    cp_async_wait<0>();
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&kv_full[s]);
+                }
+            }
+        }
+        if (abort_flag)  // after a wait that gave up: the copies under way end (or are given up) before the memory is left
+            for (int i = max(0, g - kStages); i < g; ++i)
+                if (!mbar_wait(&kv_full[i % kStages], unsigned((i / kStages) & 1), p.error)) break;
+    } else if (warp == 10) {
+        // ---- Q
+        int loads[2] = {0, 0};
+        while (!abort_flag && cursor.next(p, total, w)) {
+            if (!w.tiles) continue;
+            for (int k = 0; k < w.active && !abort_flag; ++k) {
+                if (!mbar_wait(&q_empty[k], unsigned(loads[k] & 1) ^ 1, p.error)) abort_flag = 1;
+                if (abort_flag) break;
+                ++loads[k];
+                constexpr int kChunks = 8 * H;
+                uint8_t* to0 = Qs + k * Shape::kTile;
+                for (int e = lane; e < kPrTile * kChunks; e += 32) {
+                    const int r = e / kChunks, c = e % kChunks, row = w.row0 + k * kPrTile + r;
+                    const int token = int(p.by_group.div(row)), head = w.kvh * a.group + row - token * a.group;
+                    const bool ok = row < w.rows && c * 8 < a.dim;
+                    uint8_t* to = to0 + (c >> 3) * Shape::kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                    const auto* from = static_cast<const __nv_bfloat16*>(a.q) + (ok ? (w.token0 + token) * a.qt + head * a.qh + c * 8 : 0);
+                    if (p.q_vector)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(to)), "l"(from), "r"(ok ? 16 : 0) : "memory");
+                    else
+                        for (int i = 0; i < 8; ++i)
+                            reinterpret_cast<uint16_t*>(to)[i] = ok ? reinterpret_cast<const uint16_t*>(from)[i] : uint16_t(0);
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[k]);
+            }
+        }
+    } else if (warp == 8) {
+        // ---- products, ping-pong over the two tiles of rows
+        if (lane == 0) {
+            constexpr uint32_t idesc_s = umma_idesc_bf16(kPrTile, kPrTile);
+            constexpr uint32_t idesc_o = umma_idesc_bf16(kPrTile, D) | (1u << 16);  // B (V) MN-major
+            int g = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
+            const auto wait = [&](uint64_t* bar, int n) {
+                if (!abort_flag && !mbar_wait(bar, unsigned(n & 1), p.error)) abort_flag = 1;
+                tc_fence_after();
+                return !abort_flag;
+            };
+            const auto issue_s = [&](int k, int tile, bool last) {
+                const uint64_t dq = umma_desc_sw128(Qs + k * Shape::kTile);
+                const uint64_t dk = umma_desc_sw128(KV + (tile % kStages) * Shape::kStage);
+#pragma unroll
+                for (int c = 0; c < 4 * H; ++c) {
+                    const uint64_t off = (c >> 2) * (Shape::kBlock >> 4) + (c & 3) * 2;
+                    umma_bf16(tmem + uint32_t(k * kPrTile), dq + off, dk + off, idesc_s, c > 0);
+                }
+                umma_commit(&s_full[k]);
+                if (last) umma_commit(&q_empty[k]);
+            };
+            while (!abort_flag && cursor.next(p, total, w)) {
+                if (!w.tiles) continue;
+                bool ok = wait(&kv_full[g % kStages], g / kStages);
+                for (int k = 0; k < w.active && ok; ++k) {
+                    ok = wait(&q_full[k], q_uses[k]++);
+                    if (ok) issue_s(k, g, w.tiles == 1);
+                }
+                for (int t = 0; t < w.tiles && ok; ++t, ++g) {
+                    const uint64_t dv = umma_desc_sw128_mn(KV + (g % kStages) * Shape::kStage + Shape::kTile, Shape::kBlock);
+                    const bool more = t + 1 < w.tiles;
+                    for (int k = 0; k < w.active && ok; ++k) {
+                        ok = wait(&p_full[k], p_uses[k]++);
+                        if (!ok) break;
+                        const uint32_t tP = tmem + uint32_t(k * kPrTile), tO = tmem + uint32_t(2 * kPrTile + k * D);
+#pragma unroll
+                        for (int c = 0; c < kPrTile / 16; ++c)  // 16 keys: 8 columns of P, 2 KB down V
+                            umma_bf16_ts(tO, tP + 8 * c, dv + 128 * c, idesc_o, t > 0 || c > 0);
+                        if (!more) umma_commit(&o_done[k]);
+                        if (k == w.active - 1) umma_commit(&kv_empty[g % kStages]);
+                        if (more) {
+                            if (k == 0) ok = wait(&kv_full[(g + 1) % kStages], (g + 1) / kStages);
+                            if (ok) issue_s(k, g + 1, t + 2 == w.tiles);
+                        }
+                    }
+                }
+            }
+        }
+    } else {
+        // ---- softmax of tile k; this warp's TMEM lanes are its rows [32 q, 32 q + 32)
+        const int k = warp >> 2, q = warp & 3, r = q * 32 + lane;
+        const uint32_t lanes = uint32_t(q * 32) << 16;
+        const uint32_t tS = tmem + uint32_t(k * kPrTile) + lanes, tO = tmem + uint32_t(2 * kPrTile + k * D) + lanes;
+        int g = 0, uses = 0, ends = 0;
+        while (!abort_flag && cursor.next(p, total, w)) {
+            if (k >= w.active) {
+                g += w.tiles;
+                continue;
+            }
+            const int row = w.row0 + k * kPrTile + r, number = int(p.by_group.div(row));
+            const int token = w.token0 + number, head = w.kvh * a.group + row - number * a.group;
+            const bool row_ok = row < w.rows;
+            const int pos = row_ok ? w.pos0 + number : -1;
+            // Positions that every row of the tile sees: [max(low_all, 0), first_all].
+            const int pos_first = w.pos0 + int(p.by_group.div(w.row0 + k * kPrTile));
+            const int pos_last = w.pos0 + int(p.by_group.div(min(w.row0 + (k + 1) * kPrTile, w.rows) - 1));
+            const int end = w.pos0 + w.rows / a.group;  // rows that the slot holds
+            const int low = a.window > 0 ? pos - a.window + 1 : 0;
+            float m_run = -INFINITY, l_run = 0.f;
+            for (int t = 0; t < w.tiles; ++t, ++g) {
+                const int s = g % kStages, j0 = w.key0(t);
+                if (!mbar_wait(&s_full[k], unsigned(uses++ & 1), p.error) || !mbar_wait(&kv_full[s], unsigned((g / kStages) & 1), p.error)) abort_flag = 1;
+                if (abort_flag) break;
+                tc_fence_after();
+                uint32_t sv[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_load32_async(tS + 32 * c, sv + 32 * c);
+                const uint4 none = *reinterpret_cast<const uint4*>(gone + s * 4);
+                const bool all = j0 + kPrTile - 1 <= pos_first && (a.window <= 0 || pos_last - j0 < a.window || j0 + kPrTile <= a.first) &&
+                                 !(none.x | none.y | none.z | none.w);
+                tmem_wait_ld();
+                if (!all) {
+                    const uint32_t nw[4] = {none.x, none.y, none.z, none.w};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int base = j0 + 32 * c;
+                        const uint32_t vis = (bits_from_to(low - base, pos - base) | bits_from_to(0, min(a.first - 1, pos) - base)) & ~nw[c];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!((vis >> e) & 1)) sv[32 * c + e] = __float_as_uint(-INFINITY);
+                    }
+                    if (j0 + r >= end) {  // behind the end of the sequence: no values
+#pragma unroll
+                        for (int c = 0; c < 8 * H; ++c)
+                            *reinterpret_cast<uint4*>(KV + s * Shape::kStage + Shape::kTile + (c >> 3) * Shape::kBlock + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                }
+                float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 128; e += 8) {
+                    mq[0] = fmax3(mq[0], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+                    mq[1] = fmax3(mq[1], __uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3]));
+                    mq[2] = fmax3(mq[2], __uint_as_float(sv[e + 4]), __uint_as_float(sv[e + 5]));
+                    mq[3] = fmax3(mq[3], __uint_as_float(sv[e + 6]), __uint_as_float(sv[e + 7]));
+                }
+                const float m_tile = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) * a.scale_log2;
+                const float m_new = m_tile > m_run + 8.f ? m_tile : m_run;
+                const float corr = m_run == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+                const float neg = m_new == -INFINITY ? 0.f : -m_new;
+                const uint64_t scale2 = f32x2(a.scale_log2, a.scale_log2), neg2 = f32x2(neg, neg);
+                uint64_t sum2[2] = {f32x2(0.f, 0.f), f32x2(0.f, 0.f)};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t pw[32];
+#pragma unroll
+                    for (int u = 0; u < 32; ++u) {
+                        const uint64_t x = ffma2(f32x2(__uint_as_float(sv[64 * h + 2 * u]), __uint_as_float(sv[64 * h + 2 * u + 1])), scale2, neg2);
+                        float xa, xb;
+                        f32x2_split(x, xa, xb);
+                        xa = fast_exp2(xa);
+                        xb = fast_exp2(xb);
+                        sum2[u & 1] = fadd2(sum2[u & 1], f32x2(xa, xb));
+                        // The weights go into the product with 8 bits, as bf16 operands have; their sum keeps all.
+                        pw[u] = pack_bf16(xa, xb);
+                    }
+                    tmem_store32_async(tS + 32 * h, pw);
+                }
+                float sa, sb;
+                f32x2_split(fadd2(sum2[0], sum2[1]), sa, sb);
+                if (t > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        float ov[32];
+                        tmem_load32(tO + c * 32, ov);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) ov[e] *= corr;
+                        tmem_store32(tO + c * 32, ov);
+                    }
+                }
+                tmem_wait_st();
+                l_run = l_run * corr + (sa + sb);
+                m_run = m_new;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[k]);
+            }
+            if (abort_flag) break;
+            // ---- the item's end
+            bool again = false;
+            const float sink = row_ok ? sink_log2<__nv_bfloat16>(a.sinks, a.sinks_fp32, head) : -INFINITY;
+            const float top = fmaxf(m_run, sink);
+            const float c0 = m_run == -INFINITY ? (l_run == 0.f ? 0.f : 1.f) : fast_exp2(m_run - top);
+            const float sum = l_run * c0 + (sink == -INFINITY ? 0.f : fast_exp2(sink - top));
+            const float inv = sum == 0.f ? 0.f : c0 / sum;
+            __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(a.out) + token * a.ot + head * a.oh;
+            if (w.tiles) {
+                if (!mbar_wait(&o_done[k], unsigned(ends++ & 1), p.error)) abort_flag = 1;
+                if (abort_flag) break;
+                tc_fence_after();
+                float check = l_run * 0.f;  // NaN as soon as something is not finite
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    float ov[32];
+                    tmem_load32(tO + c * 32, ov);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) check = fmaf(ov[e], 0.f, check);
+                    if (row_ok)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            const int d = c * 32 + e;
+                            if (d >= a.dim) continue;
+                            uint32_t w4[4];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) w4[u] = pack_bf16(ov[e + 2 * u] * inv, ov[e + 2 * u + 1] * inv);
+                            if (p.out_vector) *reinterpret_cast<uint4*>(orow + d) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+                            else
+#pragma unroll
+                                for (int u = 0; u < 8; ++u) reinterpret_cast<uint16_t*>(orow + d)[u] = uint16_t(w4[u >> 1] >> (16 * (u & 1)));
+                        }
+                }
+                again = row_ok && check != 0.f;
+            } else if (row_ok) {
+                for (int d = 0; d < a.dim; ++d) orow[d] = __float2bfloat16_rn(0.f);
+            }
+            if (a.lse && row_ok) a.lse[int64_t(token) * a.heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+            for (uint32_t bad = __ballot_sync(0xffffffffu, again); bad; bad &= bad - 1) {
+                const int from = __ffs(bad) - 1;
+                const int tk = __shfl_sync(0xffffffffu, token, from), hd = __shfl_sync(0xffffffffu, head, from), ps = __shfl_sync(0xffffffffu, pos, from);
+                float m, l, o[4];
+                attend_row<__nv_bfloat16>(a, tk, hd, w.slot, ps, m, l, o);
+                __syncwarp();
+                finish_row<__nv_bfloat16>(a, tk, hd, m, l, o);
+            }
+            tc_fence_before();  // O has been read before its next products are asked for
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace cb200
