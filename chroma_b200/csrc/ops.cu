@@ -134,9 +134,9 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// Boxes of 64 values, one head, `rows` rows of one page of a bf16 pool, 128-byte swizzle. False where the pool's strides
-// are none that the TMA engine takes.
-bool page_map(CUtensorMap* map, const void* pool, const PagedArgs& a, int64_t kp, int64_t kr, int64_t kh, int rows) {
+// Tensor maps of bf16 boxes whose rows are 64 values, 128-byte swizzle; of a pool: one head, `rows` rows of one page. False
+// where the strides are none that the TMA engine takes.
+bool bf16_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
     static const EncodeTiled encode = [] {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q{};
@@ -144,14 +144,19 @@ bool page_map(CUtensorMap* map, const void* pool, const PagedArgs& a, int64_t kp
         if (!p || q != cudaDriverEntryPointSuccess) throw std::runtime_error("cuTensorMapEncodeTiled unavailable");
         return reinterpret_cast<EncodeTiled>(p);
     }();
+    const cuuint32_t step[4] = {1, 1, 1, 1};
+    for (int i = 0; i + 1 < rank; ++i)
+        if (strides[i] == 0 || strides[i] >> 40 || strides[i] % 16) return false;
+    return aligned16(base) && encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, cuuint32_t(rank), const_cast<void*>(base), dims, strides, box, step,
+                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool page_map(CUtensorMap* map, const void* pool, const PagedArgs& a, int64_t kp, int64_t kr, int64_t kh, int rows) {
     const cuuint64_t dims[4] = {cuuint64_t(a.dim), cuuint64_t(a.kv), cuuint64_t(a.page), cuuint64_t(a.pages)};
     const cuuint64_t strides[3] = {cuuint64_t(kh * 2), cuuint64_t(kr * 2), cuuint64_t(kp * 2)};
-    const cuuint32_t box[4] = {64, 1, cuuint32_t(rows), 1}, step[4] = {1, 1, 1, 1};
-    for (const cuuint64_t s : strides)
-        if (s == 0 || s >> 40) return false;
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(pool), dims, strides, box, step,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint32_t box[4] = {64, 1, cuuint32_t(rows), 1};
+    return bf16_map(map, pool, 4, dims, strides, box);
 }
 
 // How a decode is laid out, and its workspace: partial results of two items per CTA, and each CTA's join.
@@ -238,11 +243,16 @@ template <int H> void prompt_bf16(PagedPromptArgs& p, cudaStream_t s) {
     for (int rows = kPrTile; rows >= 8 && !p.box; rows /= 2)
         if (a.page % rows == 0) p.box = rows;
     if (p.box && !(page_map(&kmap, a.k, a, a.kp, a.kr, a.kh, p.box) && page_map(&vmap, a.v, a, a.vp, a.vr, a.vh, p.box))) p.box = 0;
+    CUtensorMap qmap{};
+    const cuuint64_t dims[3] = {cuuint64_t(a.dim), cuuint64_t(a.heads), cuuint64_t(a.tokens)};
+    const cuuint64_t strides[2] = {cuuint64_t(a.qh * 2), cuuint64_t(a.qt * 2)};
+    const cuuint32_t box[3] = {64, cuuint32_t(a.group), cuuint32_t(kPrTile / (a.group <= kPrTile ? a.group : kPrTile))};
+    p.q_box = kPrTile % a.group == 0 && bf16_map(&qmap, a.q, 3, dims, strides, box);
     const int64_t tiles = int64_t(a.tokens) * a.group / 256 + a.slots;  // at least as many as there are
     const int64_t items = tiles * a.kv;
     const int grid = int(items < sm_count() ? items : sm_count());
     check(cudaFuncSetAttribute(k_paged_prompt<H>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<H>::kSmem), "smem attribute");
-    launch(s, dim3(unsigned(grid)), dim3(kPrThreads), PromptShape<H>::kSmem, k_paged_prompt<H>, p, kmap, vmap);
+    launch(s, dim3(unsigned(grid)), dim3(kPrThreads), PromptShape<H>::kSmem, k_paged_prompt<H>, p, qmap, kmap, vmap);
 }
 
 void prompt(const PagedArgs& a, int storage, cudaStream_t s) {

@@ -5,14 +5,14 @@
 // query heads side by side, so that a tile of 128 rows shares every key even where a chunk has few tokens. A work item
 // is 256 consecutive rows (two tiles) of one key-value head of one sequence, against key tiles of 128 positions. The
 // grid is persistent, one CTA per SM; items are taken from the last rows of the last sequence backwards (the most keys
-// first), the key-value heads of the same rows side by side. 11 warps:
+// first), the key-value heads of the same rows side by side. 12 warps:
 //   warps 0-3, 4-7  the online softmax of tile 0, 1, one row per thread (TMEM lane = row): the row of S (128 columns)
 //                   from TMEM at once, P = 2^(s - m) back over its first 64 columns as bf16 pairs; at the item's end
 //                   O / l to global memory
 //   warp 8          one thread issues, per key tile t and tile k in turn: O_k += P_k(t) V(t), S_k(t+1) = Q_k K(t+1)^T
 //   warp 9          K and V tiles into a ring, by TMA boxes of as many rows as divide the page (a box never leaves its
 //                   page), or, where the pool or the page size is none that TMA takes, row by row with cp.async
-//   warp 10         Q tiles of the next item, as soon as the last S of this one is done
+//   warps 10, 11    Q of tile 0, 1 of the next item, as soon as the last S of this one is done
 // P stays in tensor memory as the A operand of the product with V. The tensor core runs the products of one issuing
 // thread in order, so S_k(t+1) lands over P_k(t) only after O_k has taken it, and the commit that signals S_k(t+1)
 // covers that product too: the softmax may rescale O_k as soon as it sees S_k(t+1). The maximum moves only when a tile
@@ -32,13 +32,64 @@
 
 namespace cb200 {
 
-constexpr int kPrThreads = 352, kPrTile = 128;
+constexpr int kPrThreads = 384, kPrTile = 128;
+// Registers of a softmax thread and of the others, out of the 3 x 168 that three warpgroups are launched with.
+constexpr int kPrSoftmaxRegs = 216, kPrOtherRegs = 72;
+
+// The products are issued by one elected thread of a converged warp: everything they need is the same in all lanes, so it
+// can stay in uniform registers (issued from a branch that one lane takes, a step cost up to twice its time).
+//
+// Four steps of 16 along K of D[tmem] (+)= A[smem] B[smem]^T over one 64-value block (K-major, 128-byte swizzle), as one
+// statement: the steps' descriptors are constants apart, and nothing comes between the instructions.
+__device__ __forceinline__ void umma_ss_block(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q, e;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"
+        "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+        "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, q;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(accumulate))
+        : "memory");
+}
+
+// Eight steps of 16 along K of D[tmem] (+)= P[tmem] V[smem]: P 128 x 128 (8 columns a step), V MN-major (2 KB a step).
+__device__ __forceinline__ void umma_ts_128(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q, e;\n\t.reg .b64 b1, b2, b3, b4, b5, b6, b7;\n\t.reg .b32 a1, a2, a3, a4, a5, a6, a7;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"
+        "add.s64 b1, %2, 128;\n\tadd.s64 b2, %2, 256;\n\tadd.s64 b3, %2, 384;\n\tadd.s64 b4, %2, 512;\n\t"
+        "add.s64 b5, %2, 640;\n\tadd.s64 b6, %2, 768;\n\tadd.s64 b7, %2, 896;\n\t"
+        "add.s32 a1, %1, 8;\n\tadd.s32 a2, %1, 16;\n\tadd.s32 a3, %1, 24;\n\tadd.s32 a4, %1, 32;\n\t"
+        "add.s32 a5, %1, 40;\n\tadd.s32 a6, %1, 48;\n\tadd.s32 a7, %1, 56;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a4], b4, %3, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a5], b5, %3, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a6], b6, %3, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a7], b7, %3, q;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(accumulate))
+        : "memory");
+}
+
+// Arrives on `bar` once the products that the elected thread issued before are done.
+__device__ __forceinline__ void umma_commit_elected(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
+        : "memory");
+}
 
 struct PagedPromptArgs {
     PagedArgs a;
     FastDiv by_group;
     int box;                 // rows of a TMA box; 0: row by row
     int q_vector, out_vector;  // rows are 16-byte aligned
+    int q_box;               // Q tiles come as one TMA box: `group` heads of 128 / group tokens
     unsigned* error;
 };
 
@@ -164,7 +215,8 @@ __device__ __forceinline__ uint32_t bits_from_to(int lo, int hi) {  // bits lo..
 
 template <int H>
 __global__ void __launch_bounds__(kPrThreads, 1)
-k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+               const __grid_constant__ CUtensorMap vmap) {
     using Shape = PromptShape<H>;
     constexpr int kStages = Shape::kStages, D = 64 * H;
     extern __shared__ uint8_t pr_raw[];
@@ -177,7 +229,7 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap kmap
     __shared__ int s_total;
     __shared__ volatile int abort_flag;
     const PagedArgs& a = p.a;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int k = 0; k < 2; ++k) {
@@ -213,6 +265,8 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap kmap
     PromptCursor cursor(a);
     PromptItem w;
 
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrOtherRegs));
     if (warp == 9) {
         // ---- K and V
         int g = 0;  // tiles so far
@@ -288,86 +342,93 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap kmap
         if (abort_flag)  // after a wait that gave up: the copies under way end (or are given up) before the memory is left
             for (int i = max(0, g - kStages); i < g; ++i)
                 if (!mbar_wait(&kv_full[i % kStages], unsigned((i / kStages) & 1), p.error)) break;
-    } else if (warp == 10) {
-        // ---- Q
-        int loads[2] = {0, 0};
+    } else if (warp >= 10) {
+        // ---- Q of tile `warp - 10`
+        const int k = warp - 10;
+        int loads = 0;
+        while (!abort_flag && cursor.next(p, total, w)) {
+            if (!w.tiles || k >= w.active) continue;
+            if (!mbar_wait(&q_empty[k], unsigned(loads & 1) ^ 1, p.error)) abort_flag = 1;
+            if (abort_flag) break;
+            ++loads;
+            constexpr int kChunks = 8 * H;
+            uint8_t* to0 = Qs + k * Shape::kTile;
+            const int first = w.row0 + k * kPrTile;
+            if (p.q_box) {
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&q_full[k], Shape::kTile);
+                    for (int h = 0; h < H; ++h)
+                        tma_load_3d(to0 + h * Shape::kBlock, &qmap, h * 64, w.kvh * a.group, w.token0 + int(p.by_group.div(first)), &q_full[k]);
+                }
+                continue;
+            }
+            for (int e = lane; e < kPrTile * kChunks; e += 32) {
+                const int r = e / kChunks, c = e % kChunks, row = first + r;
+                const int token = int(p.by_group.div(row)), head = w.kvh * a.group + row - token * a.group;
+                const bool ok = row < w.rows && c * 8 < a.dim;
+                uint8_t* to = to0 + (c >> 3) * Shape::kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                const auto* from = static_cast<const __nv_bfloat16*>(a.q) + (ok ? (w.token0 + token) * a.qt + head * a.qh + c * 8 : 0);
+                if (p.q_vector)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(to)), "l"(from), "r"(ok ? 16 : 0) : "memory");
+                else
+                    for (int i = 0; i < 8; ++i)
+                        reinterpret_cast<uint16_t*>(to)[i] = ok ? reinterpret_cast<const uint16_t*>(from)[i] : uint16_t(0);
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[k]);
+        }
+        if (abort_flag && loads) mbar_wait(&q_full[k], unsigned(loads - 1) & 1, p.error);
+    } else if (warp == 8) {
+        // ---- products, ping-pong over the two tiles of rows; the warp stays converged
+        constexpr uint32_t idesc_s = umma_idesc_bf16(kPrTile, kPrTile);
+        constexpr uint32_t idesc_o = umma_idesc_bf16(kPrTile, D) | (1u << 16);  // B (V) MN-major
+        int g = 0, p_uses[2] = {0, 0};
+        const auto wait = [&](uint64_t* bar, int n) {
+            const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, unsigned(n & 1), p.error));
+            if (!ok) abort_flag = 1;
+            tc_fence_after();
+            return ok;
+        };
+        const auto issue_s = [&](int k, int tile, bool last) {
+            const uint64_t dq = umma_desc_sw128(Qs + k * Shape::kTile);
+            const uint64_t dk = umma_desc_sw128(KV + (tile % kStages) * Shape::kStage);
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+                umma_ss_block(tmem + uint32_t(k * kPrTile), dq + h * (Shape::kBlock >> 4), dk + h * (Shape::kBlock >> 4), idesc_s, h > 0);
+            umma_commit_elected(&s_full[k]);
+            if (last) umma_commit_elected(&q_empty[k]);
+        };
+        int q_used[2] = {0, 0};
         while (!abort_flag && cursor.next(p, total, w)) {
             if (!w.tiles) continue;
-            for (int k = 0; k < w.active && !abort_flag; ++k) {
-                if (!mbar_wait(&q_empty[k], unsigned(loads[k] & 1) ^ 1, p.error)) abort_flag = 1;
-                if (abort_flag) break;
-                ++loads[k];
-                constexpr int kChunks = 8 * H;
-                uint8_t* to0 = Qs + k * Shape::kTile;
-                for (int e = lane; e < kPrTile * kChunks; e += 32) {
-                    const int r = e / kChunks, c = e % kChunks, row = w.row0 + k * kPrTile + r;
-                    const int token = int(p.by_group.div(row)), head = w.kvh * a.group + row - token * a.group;
-                    const bool ok = row < w.rows && c * 8 < a.dim;
-                    uint8_t* to = to0 + (c >> 3) * Shape::kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                    const auto* from = static_cast<const __nv_bfloat16*>(a.q) + (ok ? (w.token0 + token) * a.qt + head * a.qh + c * 8 : 0);
-                    if (p.q_vector)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(to)), "l"(from), "r"(ok ? 16 : 0) : "memory");
-                    else
-                        for (int i = 0; i < 8; ++i)
-                            reinterpret_cast<uint16_t*>(to)[i] = ok ? reinterpret_cast<const uint16_t*>(from)[i] : uint16_t(0);
-                }
-                cp_async_commit();
-                cp_async_wait<0>();
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[k]);
+            bool ok = wait(&kv_full[g % kStages], g / kStages);
+            for (int k = 0; k < w.active && ok; ++k) {
+                ok = wait(&q_full[k], q_used[k]++);
+                if (ok) issue_s(k, g, w.tiles == 1);
             }
-        }
-    } else if (warp == 8) {
-        // ---- products, ping-pong over the two tiles of rows
-        if (lane == 0) {
-            constexpr uint32_t idesc_s = umma_idesc_bf16(kPrTile, kPrTile);
-            constexpr uint32_t idesc_o = umma_idesc_bf16(kPrTile, D) | (1u << 16);  // B (V) MN-major
-            int g = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
-            const auto wait = [&](uint64_t* bar, int n) {
-                if (!abort_flag && !mbar_wait(bar, unsigned(n & 1), p.error)) abort_flag = 1;
-                tc_fence_after();
-                return !abort_flag;
-            };
-            const auto issue_s = [&](int k, int tile, bool last) {
-                const uint64_t dq = umma_desc_sw128(Qs + k * Shape::kTile);
-                const uint64_t dk = umma_desc_sw128(KV + (tile % kStages) * Shape::kStage);
-#pragma unroll
-                for (int c = 0; c < 4 * H; ++c) {
-                    const uint64_t off = (c >> 2) * (Shape::kBlock >> 4) + (c & 3) * 2;
-                    umma_bf16(tmem + uint32_t(k * kPrTile), dq + off, dk + off, idesc_s, c > 0);
-                }
-                umma_commit(&s_full[k]);
-                if (last) umma_commit(&q_empty[k]);
-            };
-            while (!abort_flag && cursor.next(p, total, w)) {
-                if (!w.tiles) continue;
-                bool ok = wait(&kv_full[g % kStages], g / kStages);
+            for (int t = 0; t < w.tiles && ok; ++t, ++g) {
+                const uint64_t dv = umma_desc_sw128_mn(KV + (g % kStages) * Shape::kStage + Shape::kTile, Shape::kBlock);
+                const bool more = t + 1 < w.tiles;
                 for (int k = 0; k < w.active && ok; ++k) {
-                    ok = wait(&q_full[k], q_uses[k]++);
-                    if (ok) issue_s(k, g, w.tiles == 1);
-                }
-                for (int t = 0; t < w.tiles && ok; ++t, ++g) {
-                    const uint64_t dv = umma_desc_sw128_mn(KV + (g % kStages) * Shape::kStage + Shape::kTile, Shape::kBlock);
-                    const bool more = t + 1 < w.tiles;
-                    for (int k = 0; k < w.active && ok; ++k) {
-                        ok = wait(&p_full[k], p_uses[k]++);
-                        if (!ok) break;
-                        const uint32_t tP = tmem + uint32_t(k * kPrTile), tO = tmem + uint32_t(2 * kPrTile + k * D);
-#pragma unroll
-                        for (int c = 0; c < kPrTile / 16; ++c)  // 16 keys: 8 columns of P, 2 KB down V
-                            umma_bf16_ts(tO, tP + 8 * c, dv + 128 * c, idesc_o, t > 0 || c > 0);
-                        if (!more) umma_commit(&o_done[k]);
-                        if (k == w.active - 1) umma_commit(&kv_empty[g % kStages]);
-                        if (more) {
-                            if (k == 0) ok = wait(&kv_full[(g + 1) % kStages], (g + 1) / kStages);
-                            if (ok) issue_s(k, g + 1, t + 2 == w.tiles);
-                        }
+                    ok = wait(&p_full[k], p_uses[k]++);
+                    if (!ok) break;
+                    umma_ts_128(tmem + uint32_t(2 * kPrTile + k * D), tmem + uint32_t(k * kPrTile), dv, idesc_o, t > 0);
+                    if (!more) umma_commit_elected(&o_done[k]);
+                    if (k == w.active - 1) umma_commit_elected(&kv_empty[g % kStages]);
+                    if (more) {
+                        if (k == 0) ok = wait(&kv_full[(g + 1) % kStages], (g + 1) / kStages);
+                        if (ok) issue_s(k, g + 1, t + 2 == w.tiles);
                     }
                 }
+                if (abort_flag) ok = false;
             }
         }
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPrSoftmaxRegs));
         // ---- softmax of tile k; this warp's TMEM lanes are its rows [32 q, 32 q + 32)
         const int k = warp >> 2, q = warp & 3, r = q * 32 + lane;
         const uint32_t lanes = uint32_t(q * 32) << 16;
