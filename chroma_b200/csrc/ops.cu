@@ -259,6 +259,7 @@ void prompt(const PagedArgs& a, int storage, cudaStream_t s) {
     PagedPromptArgs p{};
     p.a = a;
     p.by_group = FastDiv(uint32_t(a.group));
+    p.by_kv = FastDiv(uint32_t(a.kv));
     p.error = error_word();
     const int64_t size = int64_t(element(storage));
     p.q_vector = aligned16(a.q) && a.qt * size % 16 == 0 && a.qh * size % 16 == 0;

@@ -13,10 +13,18 @@
 //   warp 9          K and V tiles into a ring, by TMA boxes of as many rows as divide the page (a box never leaves its
 //                   page), or, where the pool or the page size is none that TMA takes, row by row with cp.async
 //   warps 10, 11    Q of tile 0, 1 of the next item, as soon as the last S of this one is done
-// P stays in tensor memory as the A operand of the product with V. The tensor core runs the products of one issuing
-// thread in order, so S_k(t+1) lands over P_k(t) only after O_k has taken it, and the commit that signals S_k(t+1)
-// covers that product too: the softmax may rescale O_k as soon as it sees S_k(t+1). The maximum moves only when a tile
-// exceeds it by more than 2^8, so O is rescaled rarely.
+// P stays in tensor memory as the A operand of the product with V. Heads of up to 64 values leave room for P beside S, so
+// that S_k(t+1) is computed while the exponentials of S_k(t) are taken. With wider heads P lies over S: the tensor core
+// runs the products of one issuing thread in order, so S_k(t+1) lands only after O_k has taken P_k(t), and the commit
+// that signals S_k(t+1) covers that product too. The maximum moves only when a tile exceeds it by more than 2^8, so O is
+// rescaled rarely.
+//
+// What bounds it: the exponentials and what goes with them on 128 rows of one thread each, in turn with the products
+// (clock stamps per tile of 64-value heads: 1,400 cycles of exponentials, 650 around them, 1,000 waiting; the
+// special-function unit is busy half of the time, the tensor core a quarter). Four prompts of 2,048 tokens, 64/8 heads of
+// 64: 300 us, 458 TFLOP/s; 8,192 tokens after 8,001 in a window of 4,096, 32/8 heads of 128: 586 us, 939 TFLOP/s. Tried
+// and slower: a quarter to a half of the exponentials as a polynomial on the FMA pipe (305 to 354 us; issue slots), the
+// issuing warp taking whatever is ready first (301 and 653 us), the two tiles' exponentials in turn (313 and 604 us).
 //
 // A position that no row may see costs nothing (whole tiles are passed over) or a mask of 128 bits per row, applied only
 // to the tiles that need it. Values behind the end of a sequence are cleared in shared memory, since what lies there may
@@ -86,7 +94,7 @@ __device__ __forceinline__ void umma_commit_elected(uint64_t* bar) {
 
 struct PagedPromptArgs {
     PagedArgs a;
-    FastDiv by_group;
+    FastDiv by_group, by_kv;
     int box;                 // rows of a TMA box; 0: row by row
     int q_vector, out_vector;  // rows are 16-byte aligned
     int q_box;               // Q tiles come as one TMA box: `group` heads of 128 / group tokens
@@ -118,11 +126,11 @@ struct PromptCursor {
     }
     __device__ __forceinline__ bool next(const PagedPromptArgs& p, int total, PromptItem& w) {
         const PagedArgs& a = p.a;
-        const int64_t i = int64_t(round) * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        const unsigned i = unsigned(round) * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         ++round;
-        if (i >= int64_t(total) * a.kv) return false;
-        const int tile = int(i / a.kv);
-        w.kvh = int(i % a.kv);
+        if (i >= unsigned(total) * unsigned(a.kv)) return false;
+        const int tile = int(p.by_kv.div(i));
+        w.kvh = int(i) - tile * a.kv;
         int rows = rows_of(a, slot), n = (rows + 255) / 256;
         while (tile >= before + n) {
             before += n;
@@ -218,13 +226,15 @@ __global__ void __launch_bounds__(kPrThreads, 1)
 k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                const __grid_constant__ CUtensorMap vmap) {
     using Shape = PromptShape<H>;
-    constexpr int kStages = Shape::kStages, D = 64 * H;
+    // TMEM columns: S of the two tiles; P of each over its S (H = 2) or in 64 columns of its own (H = 1); O.
+    constexpr bool kOwnP = H == 1;
+    constexpr int kStages = Shape::kStages, D = 64 * H, kO = 512 - 2 * D;
     extern __shared__ uint8_t pr_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pr_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* Qs = sm;                           // [2][H][128][64]
     uint8_t* KV = Qs + 2 * Shape::kTile;        // stage s: K at s * kStage, V kTile behind it
     uint32_t* gone = reinterpret_cast<uint32_t*>(KV + kStages * Shape::kStage);  // [kStages][4]
-    __shared__ uint64_t q_full[2], q_empty[2], kv_full[kStages], kv_empty[kStages], s_full[2], p_full[2], o_done[2];
+    __shared__ uint64_t q_full[2], q_empty[2], kv_full[kStages], kv_empty[kStages], s_full[2], s_free[2], p_full[2], o_done[2];
     __shared__ uint32_t tmem_base;
     __shared__ int s_total;
     __shared__ volatile int abort_flag;
@@ -236,6 +246,7 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap
             mbar_init(&q_full[k], 1);
             mbar_init(&q_empty[k], 1);
             mbar_init(&s_full[k], 1);
+            mbar_init(&s_free[k], 4);
             mbar_init(&p_full[k], 4);
             mbar_init(&o_done[k], 1);
         }
@@ -385,42 +396,54 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap
         // ---- products, ping-pong over the two tiles of rows; the warp stays converged
         constexpr uint32_t idesc_s = umma_idesc_bf16(kPrTile, kPrTile);
         constexpr uint32_t idesc_o = umma_idesc_bf16(kPrTile, D) | (1u << 16);  // B (V) MN-major
-        int g = 0, p_uses[2] = {0, 0};
+        int g = 0, q_used[2] = {0, 0}, s_used[2] = {0, 0}, p_used[2] = {0, 0};
         const auto wait = [&](uint64_t* bar, int n) {
             const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, unsigned(n & 1), p.error));
             if (!ok) abort_flag = 1;
             tc_fence_after();
             return ok;
         };
-        const auto issue_s = [&](int k, int tile, bool last) {
+        // S_k of tile t of the item: over columns that have been read (own columns for P) or whose P has been used.
+        const auto next_s = [&](int k, int tile, int t) {
+            if (kOwnP && s_used[k] && !wait(&s_free[k], s_used[k] - 1)) return false;
+            ++s_used[k];
             const uint64_t dq = umma_desc_sw128(Qs + k * Shape::kTile);
             const uint64_t dk = umma_desc_sw128(KV + (tile % kStages) * Shape::kStage);
 #pragma unroll
             for (int h = 0; h < H; ++h)
                 umma_ss_block(tmem + uint32_t(k * kPrTile), dq + h * (Shape::kBlock >> 4), dk + h * (Shape::kBlock >> 4), idesc_s, h > 0);
             umma_commit_elected(&s_full[k]);
-            if (last) umma_commit_elected(&q_empty[k]);
+            if (t + 1 == w.tiles) umma_commit_elected(&q_empty[k]);
+            return true;
         };
-        int q_used[2] = {0, 0};
+        const auto next_o = [&](int k, int tile, int t) {
+            const uint64_t dv = umma_desc_sw128_mn(KV + (tile % kStages) * Shape::kStage + Shape::kTile, Shape::kBlock);
+            if (!wait(&p_full[k], p_used[k])) return false;
+            umma_ts_128(tmem + uint32_t(kO + k * D), tmem + uint32_t(kOwnP ? 2 * kPrTile + k * 64 : k * kPrTile), dv, idesc_o, t > 0);
+            ++p_used[k];
+            if (kOwnP || t + 1 == w.tiles) umma_commit_elected(&o_done[k]);
+            if (k == w.active - 1) umma_commit_elected(&kv_empty[tile % kStages]);
+            return true;
+        };
         while (!abort_flag && cursor.next(p, total, w)) {
             if (!w.tiles) continue;
+            const bool two = w.active == 2;
             bool ok = wait(&kv_full[g % kStages], g / kStages);
-            for (int k = 0; k < w.active && ok; ++k) {
-                ok = wait(&q_full[k], q_used[k]++);
-                if (ok) issue_s(k, g, w.tiles == 1);
-            }
+            for (int k = 0; k < w.active && ok; ++k) ok = wait(&q_full[k], q_used[k]++) && next_s(k, g, 0);
             for (int t = 0; t < w.tiles && ok; ++t, ++g) {
-                const uint64_t dv = umma_desc_sw128_mn(KV + (g % kStages) * Shape::kStage + Shape::kTile, Shape::kBlock);
                 const bool more = t + 1 < w.tiles;
-                for (int k = 0; k < w.active && ok; ++k) {
-                    ok = wait(&p_full[k], p_uses[k]++);
-                    if (!ok) break;
-                    umma_ts_128(tmem + uint32_t(2 * kPrTile + k * D), tmem + uint32_t(k * kPrTile), dv, idesc_o, t > 0);
-                    if (!more) umma_commit_elected(&o_done[k]);
-                    if (k == w.active - 1) umma_commit_elected(&kv_empty[g % kStages]);
-                    if (more) {
-                        if (k == 0) ok = wait(&kv_full[(g + 1) % kStages], (g + 1) / kStages);
-                        if (ok) issue_s(k, g + 1, t + 2 == w.tiles);
+                if (kOwnP) {  // the order in which two warpgroups half a period apart get there
+                    if (more) ok = wait(&kv_full[(g + 1) % kStages], (g + 1) / kStages);
+                    if (ok && more) ok = next_s(0, g + 1, t + 1);
+                    if (ok && two && t) ok = next_o(1, g - 1, t - 1);
+                    if (ok && two && more) ok = next_s(1, g + 1, t + 1);
+                    if (ok) ok = next_o(0, g, t);
+                    if (ok && two && !more) ok = next_o(1, g, t);
+                } else {
+                    for (int k = 0; k < w.active && ok; ++k) {
+                        ok = next_o(k, g, t);
+                        if (ok && more && k == 0) ok = wait(&kv_full[(g + 1) % kStages], (g + 1) / kStages);
+                        if (ok && more) ok = next_s(k, g + 1, t + 1);
                     }
                 }
                 if (abort_flag) ok = false;
@@ -432,7 +455,8 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap
         // ---- softmax of tile k; this warp's TMEM lanes are its rows [32 q, 32 q + 32)
         const int k = warp >> 2, q = warp & 3, r = q * 32 + lane;
         const uint32_t lanes = uint32_t(q * 32) << 16;
-        const uint32_t tS = tmem + uint32_t(k * kPrTile) + lanes, tO = tmem + uint32_t(2 * kPrTile + k * D) + lanes;
+        const uint32_t tS = tmem + uint32_t(k * kPrTile) + lanes, tO = tmem + uint32_t(kO + k * D) + lanes;
+        const uint32_t tP = kOwnP ? tmem + uint32_t(2 * kPrTile + k * 64) + lanes : tS;
         int g = 0, uses = 0, ends = 0;
         while (!abort_flag && cursor.next(p, total, w)) {
             if (k >= w.active) {
@@ -448,19 +472,26 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap
             const int pos_last = w.pos0 + int(p.by_group.div(min(w.row0 + (k + 1) * kPrTile, w.rows) - 1));
             const int end = w.pos0 + w.rows / a.group;  // rows that the slot holds
             const int low = a.window > 0 ? pos - a.window + 1 : 0;
+            const float sink = row_ok ? sink_log2<__nv_bfloat16>(a.sinks, a.sinks_fp32, head) : -INFINITY;
             float m_run = -INFINITY, l_run = 0.f;
             for (int t = 0; t < w.tiles; ++t, ++g) {
                 const int s = g % kStages, j0 = w.key0(t);
-                if (!mbar_wait(&s_full[k], unsigned(uses++ & 1), p.error) || !mbar_wait(&kv_full[s], unsigned((g / kStages) & 1), p.error)) abort_flag = 1;
+                if (!mbar_wait(&kv_full[s], unsigned((g / kStages) & 1), p.error)) abort_flag = 1;
+                const uint4 none = *reinterpret_cast<const uint4*>(gone + s * 4);
+                const bool all = j0 + kPrTile - 1 <= pos_first && (a.window <= 0 || pos_last - j0 < a.window || j0 + kPrTile <= a.first) &&
+                                 !(none.x | none.y | none.z | none.w);
+                if (!mbar_wait(&s_full[k], unsigned(uses++ & 1), p.error)) abort_flag = 1;
                 if (abort_flag) break;
                 tc_fence_after();
                 uint32_t sv[128];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_load32_async(tS + 32 * c, sv + 32 * c);
-                const uint4 none = *reinterpret_cast<const uint4*>(gone + s * 4);
-                const bool all = j0 + kPrTile - 1 <= pos_first && (a.window <= 0 || pos_last - j0 < a.window || j0 + kPrTile <= a.first) &&
-                                 !(none.x | none.y | none.z | none.w);
                 tmem_wait_ld();
+                if (kOwnP) {  // S may be overwritten
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_free[k]);
+                }
                 if (!all) {
                     const uint32_t nw[4] = {none.x, none.y, none.z, none.w};
 #pragma unroll
@@ -490,24 +521,30 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap
                 const float m_new = m_tile > m_run + 8.f ? m_tile : m_run;
                 const float corr = m_run == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
                 const float neg = m_new == -INFINITY ? 0.f : -m_new;
+                m_run = m_new;
+                // P's own columns, and O, are this warpgroup's once the product before is done; without own columns, S said so.
+                // Waited for here and not before P is stored, it also keeps the two warpgroups half a period apart (300 us
+                // for the four prompts of 2,048 tokens, against 334).
+                if (kOwnP) {
+                    if (uses > 1 && !mbar_wait(&o_done[k], unsigned(uses & 1), p.error)) abort_flag = 1;
+                    tc_fence_after();
+                }
                 const uint64_t scale2 = f32x2(a.scale_log2, a.scale_log2), neg2 = f32x2(neg, neg);
                 uint64_t sum2[2] = {f32x2(0.f, 0.f), f32x2(0.f, 0.f)};
+                uint32_t pw[64];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t pw[32];
-#pragma unroll
-                    for (int u = 0; u < 32; ++u) {
-                        const uint64_t x = ffma2(f32x2(__uint_as_float(sv[64 * h + 2 * u]), __uint_as_float(sv[64 * h + 2 * u + 1])), scale2, neg2);
-                        float xa, xb;
-                        f32x2_split(x, xa, xb);
-                        xa = fast_exp2(xa);
-                        xb = fast_exp2(xb);
-                        sum2[u & 1] = fadd2(sum2[u & 1], f32x2(xa, xb));
-                        // The weights go into the product with 8 bits, as bf16 operands have; their sum keeps all.
-                        pw[u] = pack_bf16(xa, xb);
-                    }
-                    tmem_store32_async(tS + 32 * h, pw);
+                for (int u = 0; u < 64; ++u) {
+                    const uint64_t x = ffma2(f32x2(__uint_as_float(sv[2 * u]), __uint_as_float(sv[2 * u + 1])), scale2, neg2);
+                    float xa, xb;
+                    f32x2_split(x, xa, xb);
+                    xa = fast_exp2(xa);
+                    xb = fast_exp2(xb);
+                    sum2[u & 1] = fadd2(sum2[u & 1], f32x2(xa, xb));
+                    // The weights go into the product with 8 bits, as bf16 operands have; their sum keeps all.
+                    pw[u] = pack_bf16(xa, xb);
+                    if (u == 31) tmem_store32_async(tP, pw);
                 }
+                tmem_store32_async(tP + 32, pw + 32);
                 float sa, sb;
                 f32x2_split(fadd2(sum2[0], sum2[1]), sa, sb);
                 if (t > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
@@ -522,7 +559,6 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap
                 }
                 tmem_wait_st();
                 l_run = l_run * corr + (sa + sb);
-                m_run = m_new;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[k]);
@@ -530,14 +566,13 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap
             if (abort_flag) break;
             // ---- the item's end
             bool again = false;
-            const float sink = row_ok ? sink_log2<__nv_bfloat16>(a.sinks, a.sinks_fp32, head) : -INFINITY;
             const float top = fmaxf(m_run, sink);
             const float c0 = m_run == -INFINITY ? (l_run == 0.f ? 0.f : 1.f) : fast_exp2(m_run - top);
             const float sum = l_run * c0 + (sink == -INFINITY ? 0.f : fast_exp2(sink - top));
             const float inv = sum == 0.f ? 0.f : c0 / sum;
             __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(a.out) + token * a.ot + head * a.oh;
             if (w.tiles) {
-                if (!mbar_wait(&o_done[k], unsigned(ends++ & 1), p.error)) abort_flag = 1;
+                if (!mbar_wait(&o_done[k], unsigned((kOwnP ? uses - 1 : ends++) & 1), p.error)) abort_flag = 1;
                 if (abort_flag) break;
                 tc_fence_after();
                 float check = l_run * 0.f;  // NaN as soon as something is not finite
