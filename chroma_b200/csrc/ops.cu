@@ -13,6 +13,7 @@
 #include "logits.cuh"
 #include "paged.cuh"
 #include "paged_decode.cuh"
+#include "paged_fp32.cuh"
 #include "paged_prompt.cuh"
 #include "pages.cuh"
 
@@ -236,6 +237,37 @@ void decode(const PagedArgs& a, const chroma_b200_attention& g, int storage, cud
     else by_dim(std::integral_constant<int, 4>());
 }
 
+void attention_fp32(const PagedArgs& a, const chroma_b200_attention& g, cudaStream_t s) {
+    const DecodeSpace space(a.heads, a.kv, a.dim);
+    PagedDecodeArgs p{};
+    p.a = a;
+    p.blocks = (a.group + kF32Rows - 1) / kF32Rows;
+    p.least = kF32Warps;
+    const int64_t lines = int64_t(a.kv) * p.blocks, items = a.slots * lines;
+    const int per_item = a.starts && a.group < kF32Rows ? kF32Rows / a.group : 1;
+    // Single tokens are not cut where a CTA's warps have one unit each anyway, nor where there are plenty of items.
+    p.whole = a.starts || int64_t(a.width) * a.page <= 32 * kF32Warps || items >= int64_t(8) * space.grid || lines > sm_count();
+    const int64_t blocks = a.starts ? (int64_t(a.tokens) + per_item - 1) / per_item * lines : p.whole ? items : sm_count() * 2;
+    want(blocks < kMaxRows, "more than 2^30 heads");
+    if (!p.whole) {
+        want(g.workspace && g.workspace_bytes >= space.bytes, "workspace too small");
+        p.parts = static_cast<float*>(g.workspace);
+        p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(g.workspace) + space.parts);
+        p.joins = reinterpret_cast<int4*>(static_cast<char*>(g.workspace) + space.parts + space.ml);
+    }
+    const auto run = [&](auto words) {
+        constexpr int W = decltype(words)::value, DP = W * 4 < 32 ? 32 : W * 4;
+        launch(s, dim3(unsigned(blocks)), dim3(32 * kF32Warps), 0, k_paged_fp32<W>, p, per_item);
+        if (p.whole) return;
+        if (a.slots >= blocks / lines / 4) launch_after(s, dim3(unsigned(blocks), 1), dim3(256), k_paged_join<float, DP, true>, p, kF32Rows);
+        else launch_after(s, dim3(unsigned(blocks), kF32Rows), dim3(256), k_paged_join<float, DP, false>, p, kF32Rows);
+    };
+    if (a.dim <= 16) run(std::integral_constant<int, 4>());
+    else if (a.dim <= 32) run(std::integral_constant<int, 8>());
+    else if (a.dim <= 64) run(std::integral_constant<int, 16>());
+    else run(std::integral_constant<int, 32>());
+}
+
 template <int H> void prompt_bf16(PagedPromptArgs& p, cudaStream_t s) {
     const PagedArgs& a = p.a;
     CUtensorMap kmap{}, vmap{};
@@ -330,13 +362,10 @@ int chroma_b200_paged_attention(const chroma_b200_pages* p, const chroma_b200_at
         a.qt = g->q_strides[0], a.qh = g->q_strides[1], a.ot = g->out_strides[0], a.oh = g->out_strides[1];
         a.tokens = g->tokens, a.heads = g->heads, a.group = g->heads / p->kv_heads;
         a.window = g->window, a.first = g->first, a.scale_log2 = g->scale * kLog2e;
-        const int64_t rows = int64_t(g->tokens) * g->heads;
-        if (!g->starts && p->storage == CHROMA_B200_BF16) return decode(a, *g, p->storage, cudaStream_t(stream));
-        if (p->storage == CHROMA_B200_BF16) return prompt(a, p->storage, cudaStream_t(stream));
-        by_type(p->storage, [&](auto t) {
-            launch(cudaStream_t(stream), dim3(unsigned((rows + 3) / 4)), dim3(128), size_t(16) * p->head_dim,
-                   k_paged_attention_rows<decltype(t)>, a);
-        });
+        const auto s = cudaStream_t(stream);
+        if (p->storage == CHROMA_B200_FP32) attention_fp32(a, *g, s);
+        else if (g->starts) prompt(a, p->storage, s);
+        else decode(a, *g, p->storage, s);
     });
 }
 

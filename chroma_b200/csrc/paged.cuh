@@ -70,67 +70,6 @@ __device__ __forceinline__ bool sees(int p, int j, int window, int first) {
     return j <= p && (window <= 0 || p - j < window || j < first);
 }
 
-// One warp per (token, head): 32 keys at a time, one per lane, then the values of the visible ones, one after another.
-// Right for every type, shape and mask.
-template <typename T> __global__ void __launch_bounds__(128) k_paged_attention_rows(PagedArgs a) {
-    extern __shared__ float rows_q[];  // [4][dim]
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t item = int64_t(blockIdx.x) * 4 + warp;
-    if (item >= int64_t(a.tokens) * a.heads) return;
-    const int token = int(item / a.heads), head = int(item % a.heads), kvh = head / a.group;
-    const int slot = a.starts ? slot_of(a.starts, a.slots, token) : token;
-    if (slot < 0) return;
-    const int len = held_rows(a.lengths, slot, a.width, a.page);
-    const int pos = a.starts ? len - a.starts[slot + 1] + token : len - 1;
-    float* q = rows_q + warp * a.dim;
-    const T* qrow = static_cast<const T*>(a.q) + token * a.qt + head * a.qh;
-    for (int d = lane; d < a.dim; d += 32) q[d] = Store<T>::load(qrow + d);
-    __syncwarp();
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    const int low = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    const int first = min(a.first, low);  // [0, first) then [low, pos]
-    const int total = max(0, pos + 1 - low + first);
-    for (int base = 0; base < total; base += 32) {
-        const int i = base + lane;
-        const int j = i < first ? i : low + i - first;
-        const int entry = i < total ? int(a.by_page.div(uint32_t(j))) : 0;
-        int id = i < total ? a.table[slot * a.ts + entry] : -1;
-        if (id >= a.pages) id = -1;
-        float s = -INFINITY;
-        const int row = j - entry * a.page;
-        if (id >= 0) {
-            const T* k = static_cast<const T*>(a.k) + id * a.kp + row * a.kr + kvh * a.kh;
-            float dot = 0.f;
-            for (int d = 0; d < a.dim; ++d) dot = fmaf(q[d], Store<T>::load(k + d), dot);
-            s = dot * a.scale_log2;
-        }
-        const float mx = fmaxf(m, warp_max(s));
-        if (mx == -INFINITY && !__any_sync(0xffffffffu, id >= 0 && isnan(s))) continue;
-        const float corr = m == -INFINITY ? 0.f : exp2f(m - mx);
-        const float p = id < 0 ? 0.f : exp2f(s - mx);
-        l = l * corr + warp_sum(p);
-        m = mx;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] *= corr;
-        for (int e = 0; e < min(32, total - base); ++e) {
-            const int ide = __shfl_sync(0xffffffffu, id, e), rowe = __shfl_sync(0xffffffffu, row, e);
-            const float pe = __shfl_sync(0xffffffffu, p, e);
-            if (ide < 0) continue;
-            const T* v = static_cast<const T*>(a.v) + ide * a.vp + rowe * a.vr + kvh * a.vh;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (c * 32 + lane < a.dim) o[c] = fmaf(pe, Store<T>::load(v + c * 32 + lane), o[c]);
-        }
-    }
-    const float sink = sink_log2<T>(a.sinks, a.sinks_fp32, head);
-    const float top = fmaxf(m, sink);
-    const float c = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - top);
-    const float sum = l * c + (sink == -INFINITY ? 0.f : exp2f(sink - top));
-    T* orow = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
-    for (int d = lane; d < a.dim; d += 32) Store<T>::store(orow + d, sum == 0.f ? 0.f : o[d >> 5] * c / sum);
-    if (a.lse && lane == 0) a.lse[item] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
-}
-
 struct AppendArgs {
     const void *nk, *nv;
     int64_t nkt, nkh, nvt, nvh;     // elements between tokens, heads of the new rows

@@ -38,9 +38,12 @@ template <int U> struct SeenUnits {
     int pos = -1, pre = 0, main0 = 0, units = 1;  // a slot with nothing to see has one unit with no visible key
     __device__ SeenUnits() {}
     __device__ SeenUnits(const PagedArgs& a, int slot) {
-        pos = held_rows(a.lengths, slot, a.width, a.page) - 1;
-        if (pos < 0) return;
-        const int low = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+        const int last = held_rows(a.lengths, slot, a.width, a.page) - 1;
+        if (last >= 0) set(a, last, last);
+    }
+    __device__ __forceinline__ void set(const PagedArgs& a, int at, int last) {  // tokens at positions at .. last
+        pos = last;
+        const int low = a.window > 0 ? max(0, at - a.window + 1) : 0;
         pre = (min(a.first, low) + U - 1) / U;
         main0 = max(low / U, pre);
         units = pre + pos / U - main0 + 1;
