@@ -63,7 +63,7 @@ def process_logits(logits: Tensor, *, history: Tensor | None = None, lengths: Te
                          f"{list(logits.shape)}")
     rows, vocab = logits.shape
     if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty((rows, vocab))
     elif out.shape != logits.shape or out.dtype is not logits.dtype or out.stride(1) != 1 \
             or (out.stride(0) < vocab and rows > 1):
         raise ValueError(f"out must be {list(logits.shape)} {logits.dtype} with contiguous rows")
@@ -84,15 +84,17 @@ def process_logits(logits: Tensor, *, history: Tensor | None = None, lengths: Te
         strides[2] = _matrix(bias, torch.float32, rows, biases, "bias")
     if mask is not None:
         strides[3] = _matrix(mask, torch.int32, rows, (vocab + 31) // 32, "mask")
-    best = torch.empty(rows, dtype=torch.int64, device=logits.device) if argmax else None
-    size = nat.lib().chroma_b200_logits_workspace(rows, vocab) if argmax else 0
-    room = torch.empty(size, dtype=torch.uint8, device=logits.device) if size else None
+    best, room, size = None, 0, 0
+    if argmax:
+        size = nat.lib().chroma_b200_logits_workspace(rows, vocab)
+        whole = torch.empty(rows + size // 8, dtype=torch.int64, device=logits.device)  # and the workspace behind the ids
+        best, room = whole[:rows], whole.data_ptr() + 8 * rows
     args = _LOGITS.pack(
         logits.data_ptr(), out.data_ptr(), 0 if best is None else best.data_ptr(), *pointers,
         _floats(repetition, rows, "repetition"), _floats(presence, rows, "presence"),
         _floats(frequency, rows, "frequency"), _floats(temperature, rows, "temperature"),
         0 if bias_ids is None else bias_ids.data_ptr(), 0 if bias is None else bias.data_ptr(),
-        0 if mask is None else mask.data_ptr(), 0 if room is None else room.data_ptr(), logits.stride(0), out.stride(0),
+        0 if mask is None else mask.data_ptr(), room, logits.stride(0), out.stride(0),
         *strides, size, storage, rows, vocab, width, biases)
     _launch(index, "chroma_b200_process_logits", args)
     return out if best is None else (out, best)

@@ -106,7 +106,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "chroma_b200_graph_destroy": (None, [_VP]),
     "chroma_b200_paged_append": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _I32, _VP, _CP, _SZ]),
     "chroma_b200_paged_attention": (ctypes.c_int, [_VP, _VP, _VP, _CP, _SZ]),
-    "chroma_b200_attention_workspace": (ctypes.c_int64, [_I32, _I32, _I32, _I32]),
+    "chroma_b200_attention_workspace": (ctypes.c_int64, [_VP, _VP]),
     "chroma_b200_step_pages": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_int64, _VP, _CP, _SZ]),
     "chroma_b200_compact_pages": (ctypes.c_int, [_VP, _VP, _VP, _VP, ctypes.c_int64, _VP, _CP, _SZ]),
     "chroma_b200_pages_workspace": (ctypes.c_int64, [_I32, _I32]),
@@ -159,8 +159,9 @@ _local = threading.local()
 
 def call_op(name: str, *args: Any) -> None:
     """``call`` for operators that run every few microseconds: one message buffer per thread."""
-    err = getattr(_local, "err", None)
-    if err is None:
+    try:
+        err = _local.err
+    except AttributeError:
         err = _local.err = ctypes.create_string_buffer(1024)
     status = getattr(_lib or lib(), name)(*args, err, 1024)
     if status != OK:

@@ -34,29 +34,22 @@ _ATTENTION = struct.Struct("=6Q5q5if")  # chroma_b200_attention
 _NEW_STRIDES = struct.Struct("=4q")
 
 
-def _need(ok: bool, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
-
-
 def _device(first: Any, *others: Any) -> int:
     """The one CUDA device of these tensors (None among them is passed over)."""
-    if not isinstance(first, Tensor):
-        raise TypeError(f"not a tensor: {type(first).__name__}")
-    index = first.get_device()
-    _need(index >= 0, "tensors must be on a CUDA device")
-    for t in others:
-        if t is None:
-            continue
-        if not isinstance(t, Tensor):
-            raise TypeError(f"not a tensor: {type(t).__name__}")
-        if t.get_device() != index:
-            raise ValueError("tensors on different devices")
+    try:
+        index = first.get_device()
+        if index < 0:
+            raise ValueError("tensors must be on a CUDA device")
+        for t in others:
+            if t is not None and t.get_device() != index:
+                raise ValueError("tensors on different devices")
+    except AttributeError:
+        raise TypeError("not a tensor among the arguments that have to be tensors") from None
     return index
 
 
 def _ints(t: Tensor, shape: tuple[int, ...], name: str) -> int:
-    if t.dtype is not torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
     return t.data_ptr()
 
@@ -73,18 +66,19 @@ def _pages(keys: Tensor, values: Tensor, table: Tensor, lengths: Tensor, layered
                          f"{list(shape)} and {list(values.shape)}")
     if ks[-1] != 1 or vs[-1] != 1:
         raise ValueError("a head's row must be contiguous")
-    if rank == 4:
-        shape, ks, vs = (1, *shape), (0, *ks), (0, *vs)
-    if table.dtype is not torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+    table_shape, ts = table.shape, table.stride()
+    if table.dtype is not torch.int32 or len(ts) != 2 or ts[1] != 1:
         raise ValueError("table must be int32 [slots, width] with contiguous rows")
-    slots, width = table.shape
-    return _PAGES.pack(keys.data_ptr(), values.data_ptr(), table.data_ptr(), _ints(lengths, (slots,), "lengths"),
-                       *ks[:4], *vs[:4], table.stride(0), storage, *shape, slots, width)
+    slots, width = table_shape
+    pointers = keys.data_ptr(), values.data_ptr(), table.data_ptr(), _ints(lengths, (slots,), "lengths")
+    if rank == 4:
+        return _PAGES.pack(*pointers, 0, ks[0], ks[1], ks[2], 0, vs[0], vs[1], vs[2], ts[0], storage, 1, *shape, slots, width)
+    return _PAGES.pack(*pointers, *ks[:4], *vs[:4], ts[0], storage, *shape, slots, width)
 
 
 def _launch(index: int, name: str, *args: Any) -> None:
     """Calls the native operator on the device's current stream; ``args`` end before the stream."""
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         nat.call_op(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -138,7 +132,7 @@ def paged_attention(q: Tensor, keys: Tensor, values: Tensor, table: Tensor, leng
     if q.dtype is not keys.dtype or dim != keys.shape[3]:
         raise ValueError(f"q must be [tokens, heads, {keys.shape[3]}] {keys.dtype}, got {list(q.shape)} {q.dtype}")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype is not q.dtype:
         raise ValueError(f"out must be {list(q.shape)} {q.dtype}, got {list(out.shape)} {out.dtype}")
     qs, os = q.stride(), out.stride()
@@ -152,12 +146,15 @@ def paged_attention(q: Tensor, keys: Tensor, values: Tensor, table: Tensor, leng
         fp32 = int(sinks.dtype is torch.float32)
     if window < 0 or first < 0:
         raise ValueError(f"window and first must be nonnegative, got {window} and {first}")
-    size = nat.lib().chroma_b200_attention_workspace(tokens, heads, keys.shape[2], dim)
-    room = torch.empty(size, dtype=torch.uint8, device=q.device) if size > 0 else None
-    args = _ATTENTION.pack(
+    fields = (
         q.data_ptr(), out.data_ptr(), 0 if logs is None else logs.data_ptr(), 0 if sinks is None else sinks.data_ptr(),
-        0 if starts is None else _ints(starts, (table.shape[0] + 1,), "starts"), 0 if room is None else room.data_ptr(),
-        size, qs[0], qs[1], os[0], os[1], tokens, heads, fp32, window, first, dim**-0.5 if scale is None else scale)
+        0 if starts is None else _ints(starts, (table.shape[0] + 1,), "starts"))
+    more = (qs[0], qs[1], os[0], os[1], tokens, heads, fp32, window, first, dim**-0.5 if scale is None else scale)
+    args = _ATTENTION.pack(*fields, 0, 0, *more)
+    size = nat.lib().chroma_b200_attention_workspace(pages, args)
+    if size > 0:
+        room = torch.empty(size, dtype=torch.uint8, device=q.device)
+        args = _ATTENTION.pack(*fields, room.data_ptr(), size, *more)
     _launch(index, "chroma_b200_paged_attention", pages, args)
     return out if logs is None else (out, logs)
 
@@ -177,14 +174,13 @@ def step_pages(table: Tensor, lengths: Tensor, parents: Tensor, counts: Tensor, 
     index = _device(keys, values, table, lengths, parents, counts)
     pages = _pages(keys, values, table, lengths, True)
     slots, width = table.shape
-    results = (torch.empty((slots, width), dtype=torch.int32, device=table.device),
-               torch.empty(slots, dtype=torch.int32, device=table.device),
-               torch.empty(3, dtype=torch.int32, device=table.device))
+    new_table, new_lengths = table.new_empty((slots, width)), torch.empty_like(lengths)
     size = nat.lib().chroma_b200_pages_workspace(keys.shape[-4], slots)
-    room = torch.empty(size, dtype=torch.uint8, device=table.device)
+    room = lengths.new_empty(3 + size // 4)  # info, and the native code's workspace behind it
+    at = room.data_ptr()
     _launch(index, "chroma_b200_step_pages", pages, _ints(parents, (slots,), "parents"),
-            _ints(counts, (slots,), "counts"), *(t.data_ptr() for t in results), room.data_ptr(), size)
-    return results
+            _ints(counts, (slots,), "counts"), new_table.data_ptr(), new_lengths.data_ptr(), at, at + 12, size)
+    return new_table, new_lengths, room[:3]
 
 
 def compact_pages(table: Tensor, lengths: Tensor, keys: Tensor, values: Tensor) -> tuple[Tensor, Tensor]:
@@ -194,9 +190,9 @@ def compact_pages(table: Tensor, lengths: Tensor, keys: Tensor, values: Tensor) 
     index = _device(keys, values, table, lengths)
     pages = _pages(keys, values, table, lengths, True)
     slots, width = table.shape
-    new_table = torch.empty((slots, width), dtype=torch.int32, device=table.device)
-    info = torch.empty(2, dtype=torch.int32, device=table.device)
+    new_table = table.new_empty((slots, width))
     size = nat.lib().chroma_b200_pages_workspace(keys.shape[-4], slots)
-    room = torch.empty(size, dtype=torch.uint8, device=table.device)
-    _launch(index, "chroma_b200_compact_pages", pages, new_table.data_ptr(), info.data_ptr(), room.data_ptr(), size)
-    return new_table, info
+    room = lengths.new_empty(2 + size // 4)  # info, and the native code's workspace behind it
+    at = room.data_ptr()
+    _launch(index, "chroma_b200_compact_pages", pages, new_table.data_ptr(), at, at + 8, size)
+    return new_table, room[:2]

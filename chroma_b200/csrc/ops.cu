@@ -4,6 +4,7 @@
 
 #include <cuda.h>
 
+#include <atomic>
 #include <cstdio>
 #include <stdexcept>
 #include <string>
@@ -76,10 +77,22 @@ void launch_after(cudaStream_t s, dim3 grid, dim3 block, void (*kernel)(Params..
     check(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...), "kernel launch");
 }
 
-int sm_count() {
-    int device = 0, n = 0;
+constexpr int kDevices = 64;
+
+int current_device() {
+    int device = 0;
     check(cudaGetDevice(&device), "device");
-    check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device), "device attribute");
+    return device;
+}
+
+int sm_count() {
+    static std::atomic<int> known[kDevices];
+    const int device = current_device();
+    int n = device < kDevices ? known[device].load(std::memory_order_relaxed) : 0;
+    if (!n) {
+        check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device), "device attribute");
+        if (device < kDevices) known[device].store(n, std::memory_order_relaxed);
+    }
     return n;
 }
 
@@ -98,6 +111,8 @@ void check_pages(const chroma_b200_pages* p) {
     want(p->head_dim > 0 && p->head_dim * size % 16 == 0 && p->head_dim <= 128,
          "head_dim: at most 128, and a multiple of 16 bytes");
     want(int64_t(p->width) * p->page_rows <= kMaxRows, "a table of more than 2^30 positions");
+    want(int64_t(p->page_rows) * p->kv_heads * p->head_dim * size <= (int64_t(1) << 29), "a page of more than 512 MB");
+    want(int64_t(p->pages) * p->layers < (int64_t(1) << 30), "more than 2^30 pages in all layers");
     want(aligned16(p->keys) && aligned16(p->values), "pools must be 16-byte aligned");
     for (int i = 0; i < 4; ++i)
         want(p->key_strides[i] * size % 16 == 0 && p->value_strides[i] * size % 16 == 0,
@@ -119,6 +134,7 @@ PoolArgs pool_args(const chroma_b200_pages& p) {
     a.layers = p.layers;
     a.heads = p.kv_heads;
     a.run = int(p.head_dim / per);
+    if (a.kh == a.run && a.vh == a.run) a.run *= a.heads, a.heads = 1, a.kh = a.vh = a.run;  // a row is one run
     return a;
 }
 
@@ -126,8 +142,13 @@ PoolArgs pool_args(const chroma_b200_pages& p) {
 __device__ unsigned g_error;
 
 unsigned* error_word() {
-    void* at = nullptr;
-    check(cudaGetSymbolAddress(&at, g_error), "error word");
+    static std::atomic<void*> known[kDevices];
+    const int device = current_device();
+    void* at = device < kDevices ? known[device].load(std::memory_order_relaxed) : nullptr;
+    if (!at) {
+        check(cudaGetSymbolAddress(&at, g_error), "error word");
+        if (device < kDevices) known[device].store(at, std::memory_order_relaxed);
+    }
     return static_cast<unsigned*>(at);
 }
 
@@ -160,13 +181,14 @@ bool page_map(CUtensorMap* map, const void* pool, const PagedArgs& a, int64_t kp
     return bf16_map(map, pool, 4, dims, strides, box);
 }
 
-// How a decode is laid out, and its workspace: partial results of two items per CTA, and each CTA's join.
+// How single tokens are laid out, and their workspace: partial results of two items per CTA, and each CTA's join.
 struct DecodeSpace {
-    int grid, tiles, pad, blocks;  // CTAs at most, tiles of 8 heads in an item, padded head row, items per kv head
+    int grid, tiles, pad, blocks, storage;  // CTAs at most, tiles of 8 heads in an item, padded head row, items per kv head
     int64_t parts, ml, bytes;
-    DecodeSpace(int heads, int kv, int dim) {
+    DecodeSpace(int heads, int kv, int dim, int type) {
         const int group = heads / kv;
-        tiles = group > 8 ? 2 : 1;
+        storage = type;
+        tiles = group > 8 && storage == CHROMA_B200_BF16 ? 2 : 1;
         pad = dim <= 32 ? 32 : dim <= 64 ? 64 : 128;
         blocks = (group + 8 * tiles - 1) / (8 * tiles);
         grid = sm_count() * 4;
@@ -174,6 +196,17 @@ struct DecodeSpace {
         parts = rows * pad * 4;
         ml = rows * 8;
         bytes = parts + ml + int64_t(grid) * 16;
+    }
+    // One CTA per item where its warps have one or two units anyway, where there are so many items that they even out,
+    // and where the heads alone outnumber the CTAs; prompts have an item per rows in fp32, and no cuts.
+    bool whole(int slots, int kv, int64_t positions, const void* starts) const {
+        return starts || positions <= 256 || int64_t(slots) * kv * blocks >= int64_t(8) * grid || int64_t(kv) * blocks > sm_count();
+    }
+    void place(PagedDecodeArgs& p, const chroma_b200_attention& g) const {
+        want(g.workspace && g.workspace_bytes >= bytes, "workspace too small");
+        p.parts = static_cast<float*>(g.workspace);
+        p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(g.workspace) + parts);
+        p.joins = reinterpret_cast<int4*>(static_cast<char*>(g.workspace) + parts + ml);
     }
 };
 
@@ -208,26 +241,19 @@ template <int DC, int NT> void decode_bf16(PagedDecodeArgs& p, int64_t items, cu
 }
 
 void decode(const PagedArgs& a, const chroma_b200_attention& g, int storage, cudaStream_t s) {
-    const DecodeSpace space(a.heads, a.kv, a.dim);
+    const DecodeSpace space(a.heads, a.kv, a.dim, storage);
     PagedDecodeArgs p{};
     p.a = a;
     p.blocks = space.blocks;
     p.error = error_word();
     const int64_t lines = int64_t(a.kv) * p.blocks, items = a.slots * lines;
     want(items < kMaxRows, "more than 2^30 heads");
-    // One CTA per item where a warp has at most four units of 16 anyway, where there are so many items that they even
-    // out, and where the heads alone outnumber the CTAs.
-    p.whole = int64_t(a.width) * a.page <= 256 || items >= int64_t(8) * space.grid || lines > sm_count();
+    p.whole = space.whole(a.slots, a.kv, int64_t(a.width) * a.page, a.starts);
     const int64_t size = int64_t(element(storage));
     p.full = a.dim == space.pad;
     p.kp = a.kp * size, p.kr = a.kr * size, p.vp = a.vp * size, p.vr = a.vr * size;
     p.q_vector = aligned16(a.q) && a.qt * size % 16 == 0 && a.qh * size % 16 == 0;
-    if (!p.whole) {
-        want(g.workspace && g.workspace_bytes >= space.bytes, "workspace too small");
-        p.parts = static_cast<float*>(g.workspace);
-        p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(g.workspace) + space.parts);
-        p.joins = reinterpret_cast<int4*>(static_cast<char*>(g.workspace) + space.parts + space.ml);
-    }
+    if (!p.whole) space.place(p, g);
     const auto by_dim = [&](auto dc) {
         if (space.tiles == 2) decode_bf16<decltype(dc)::value, 2>(p, items, s);
         else decode_bf16<decltype(dc)::value, 1>(p, items, s);
@@ -238,23 +264,17 @@ void decode(const PagedArgs& a, const chroma_b200_attention& g, int storage, cud
 }
 
 void attention_fp32(const PagedArgs& a, const chroma_b200_attention& g, cudaStream_t s) {
-    const DecodeSpace space(a.heads, a.kv, a.dim);
+    const DecodeSpace space(a.heads, a.kv, a.dim, CHROMA_B200_FP32);
     PagedDecodeArgs p{};
     p.a = a;
-    p.blocks = (a.group + kF32Rows - 1) / kF32Rows;
+    p.blocks = space.blocks;
     p.least = kF32Warps;
     const int64_t lines = int64_t(a.kv) * p.blocks, items = a.slots * lines;
     const int per_item = a.starts && a.group < kF32Rows ? kF32Rows / a.group : 1;
-    // Single tokens are not cut where a CTA's warps have one unit each anyway, nor where there are plenty of items.
-    p.whole = a.starts || int64_t(a.width) * a.page <= 32 * kF32Warps || items >= int64_t(8) * space.grid || lines > sm_count();
+    p.whole = space.whole(a.slots, a.kv, int64_t(a.width) * a.page, a.starts);
     const int64_t blocks = a.starts ? (int64_t(a.tokens) + per_item - 1) / per_item * lines : p.whole ? items : sm_count() * 2;
     want(blocks < kMaxRows, "more than 2^30 heads");
-    if (!p.whole) {
-        want(g.workspace && g.workspace_bytes >= space.bytes, "workspace too small");
-        p.parts = static_cast<float*>(g.workspace);
-        p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(g.workspace) + space.parts);
-        p.joins = reinterpret_cast<int4*>(static_cast<char*>(g.workspace) + space.parts + space.ml);
-    }
+    if (!p.whole) space.place(p, g);
     const auto run = [&](auto words) {
         constexpr int W = decltype(words)::value, DP = W * 4 < 32 ? 32 : W * 4;
         launch(s, dim3(unsigned(blocks)), dim3(32 * kF32Warps), 0, k_paged_fp32<W>, p, per_item);
@@ -300,6 +320,23 @@ void prompt(const PagedArgs& a, int storage, cudaStream_t s) {
     else prompt_bf16<2>(p, s);
 }
 
+// `list` and `count` as the launch before leaves them on the device.
+void copy_pages(const chroma_b200_pages& p, const int* list, const int* count, cudaStream_t s) {
+    const PoolArgs a = pool_args(p);
+    const int64_t parts = (int64_t(p.page_rows) * a.heads * a.run + 1023) / 1024;
+    const int64_t columns = (8 * sm_count() + parts - 1) / parts;
+    launch_after(s, dim3(unsigned(columns), unsigned(parts)), dim3(256), k_pages_copy, a, list, count);
+}
+
+// One CTA decides about pages whose marks fit its shared memory and whose table it reads in a few rounds.
+bool one_cta(const chroma_b200_pages& p) { return p.pages <= 48 * 1024 && int64_t(p.slots) * p.width <= 64 * 1024; }
+
+template <typename K> size_t shared_marks(K kernel, const chroma_b200_pages& p) {
+    const size_t bytes = size_t(p.pages) * 4;
+    if (bytes > 48 * 1024) check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)), "smem attribute");
+    return bytes;
+}
+
 dim3 table_grid(const chroma_b200_pages& p) { return dim3(unsigned((p.width + 255) / 256), unsigned(p.slots)); }
 
 }  // namespace
@@ -324,16 +361,20 @@ int chroma_b200_paged_append(const chroma_b200_pages* p, const void* new_keys, c
         a.table = p->table, a.ts = p->table_stride, a.lengths = p->lengths, a.starts = starts;
         a.slots = p->slots, a.width = p->width, a.pages = p->pages, a.page = p->page_rows, a.kv = p->kv_heads;
         a.dim = p->head_dim, a.tokens = tokens, a.by_page = FastDiv(uint32_t(p->page_rows));
+        const int64_t size = int64_t(element(p->storage));
+        int vector = aligned16(new_keys) && aligned16(new_values);
+        for (int i = 0; i < 4; ++i) vector = vector && new_strides[i] * size % 16 == 0;
         by_type(p->storage, [&](auto t) {
-            launch(cudaStream_t(stream), dim3(unsigned(tokens)), dim3(128), 0, k_paged_append<decltype(t)>, a);
+            launch(cudaStream_t(stream), dim3(unsigned((tokens + kAppendTokens - 1) / kAppendTokens)), dim3(256), 0, k_paged_append<decltype(t)>, a, vector);
         });
     });
 }
 
-int64_t chroma_b200_attention_workspace(int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim) {
-    if (tokens < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return -1;
+int64_t chroma_b200_attention_workspace(const chroma_b200_pages* p, const chroma_b200_attention* g) {
+    if (!p || !g || g->heads <= 0 || p->kv_heads <= 0 || g->heads % p->kv_heads || p->head_dim <= 0) return -1;
     try {
-        return DecodeSpace(heads, kv_heads, head_dim).bytes;
+        const DecodeSpace space(g->heads, p->kv_heads, p->head_dim, p->storage);
+        return space.whole(p->slots, p->kv_heads, int64_t(p->width) * p->page_rows, g->starts) ? 0 : space.bytes;
     } catch (...) {
         return -1;
     }
@@ -370,7 +411,7 @@ int chroma_b200_paged_attention(const chroma_b200_pages* p, const chroma_b200_at
 }
 
 int64_t chroma_b200_pages_workspace(int32_t pages, int32_t slots) {
-    return pages < 0 || slots < 0 ? -1 : (5 * int64_t(pages) + 3 * int64_t(slots) + 4) * 4;
+    return pages < 0 || slots < 0 ? -1 : (4 * int64_t(pages) + 3 * int64_t(slots) + 4) * 4;
 }
 
 int chroma_b200_step_pages(const chroma_b200_pages* p, const int32_t* parents, const int32_t* counts, int32_t* new_table,
@@ -390,10 +431,13 @@ int chroma_b200_step_pages(const chroma_b200_pages* p, const int32_t* parents, c
         a.free_list = static_cast<int*>(workspace) + p->pages;
         a.copies = a.free_list + p->pages;
         a.slots = p->slots, a.width = p->width, a.pages = p->pages, a.page = p->page_rows;
-        check(cudaMemsetAsync(a.keeper, 0, size_t(p->pages) * 4, s), "memset");
-        launch(s, table_grid(*p), dim3(256), 0, k_pages_gather, a);
-        launch(s, dim3(1), dim3(1024), 0, k_pages_assign, a);
-        launch(s, dim3(592), dim3(256), 0, k_pages_copy, pool_args(*p), a.copies, a.copies + 3 * p->slots);
+        if (one_cta(*p)) launch(s, dim3(1), dim3(1024), shared_marks(k_pages_step, *p), k_pages_step, a);
+        else {
+            check(cudaMemsetAsync(a.keeper, 0, size_t(p->pages) * 4, s), "memset");
+            launch(s, table_grid(*p), dim3(256), 0, k_pages_gather, a);
+            launch(s, dim3(1), dim3(1024), 0, k_pages_assign, a);
+        }
+        copy_pages(*p, a.copies, a.copies + 3 * p->slots, s);
     });
 }
 
@@ -409,19 +453,21 @@ int chroma_b200_compact_pages(const chroma_b200_pages* p, int32_t* new_table, in
         a.table = p->table, a.ts = p->table_stride, a.lengths = p->lengths;
         a.new_table = new_table, a.info = info;
         a.held = static_cast<unsigned*>(workspace);
-        a.to = static_cast<int*>(workspace) + p->pages;
-        a.copies = a.to + p->pages;
+        a.copies = static_cast<int*>(workspace) + p->pages;
         a.slots = p->slots, a.width = p->width, a.pages = p->pages, a.page = p->page_rows;
-        check(cudaMemsetAsync(a.held, 0, size_t(p->pages) * 4, s), "memset");
-        launch(s, table_grid(*p), dim3(256), 0, k_compact_mark, a);
-        launch(s, dim3(1), dim3(1024), 0, k_compact_plan, a);
-        launch(s, dim3(1184), dim3(256), 0, k_pages_copy, pool_args(*p), a.copies, a.copies + 3 * p->pages);
-        launch(s, table_grid(*p), dim3(256), 0, k_compact_table, a);
+        if (one_cta(*p)) launch(s, dim3(1), dim3(1024), shared_marks(k_compact, *p), k_compact, a);
+        else {
+            check(cudaMemsetAsync(a.held, 0, size_t(p->pages) * 4, s), "memset");
+            launch(s, table_grid(*p), dim3(256), 0, k_compact_mark, a);
+            launch(s, dim3(1), dim3(1024), 0, k_compact_plan, a);
+            launch(s, table_grid(*p), dim3(256), 0, k_compact_table, a);
+        }
+        copy_pages(*p, a.copies, a.copies + 3 * p->pages, s);
     });
 }
 
 int64_t chroma_b200_logits_workspace(int32_t rows, int32_t vocab) {
-    return rows < 0 || vocab < 0 ? -1 : int64_t(rows) * ((vocab + kLogitsSegment - 1) / kLogitsSegment) * 8;
+    return rows < 0 || vocab < 0 ? -1 : int64_t(rows) * ((int64_t(vocab) + kLogitsShort - 1) / kLogitsShort) * 8;
 }
 
 int chroma_b200_process_logits(const chroma_b200_logits* g, void* stream, char* err, size_t err_len) {
@@ -444,11 +490,17 @@ int chroma_b200_process_logits(const chroma_b200_logits* g, void* stream, char* 
         a.stride = g->stride, a.out_stride = g->out_stride, a.history_stride = g->history_stride;
         a.bias_ids_stride = g->bias_ids_stride, a.bias_stride = g->bias_stride, a.mask_stride = g->mask_stride;
         a.vocab = g->vocab, a.width = g->width, a.biases = g->biases;
-        a.segments = (g->vocab + kLogitsSegment - 1) / kLogitsSegment;
+        const int64_t size = int64_t(element(g->storage));
+        a.vector = aligned16(g->logits) && aligned16(g->out) && (g->rows == 1 || (g->stride * size % 16 == 0 && g->out_stride * size % 16 == 0));
+        // Long segments once they alone give every SM two CTAs.
+        const bool few = int64_t(g->rows) * ((g->vocab + kLogitsLong - 1) / kLogitsLong) < 2 * sm_count();
+        const int segment = few ? kLogitsShort : kLogitsLong;
+        a.segments = (g->vocab + segment - 1) / segment;
         by_type(g->storage, [&](auto t) {
-            launch(s, dim3(unsigned(a.segments), unsigned(g->rows)), dim3(256), 0, k_logits<decltype(t)>, a);
+            const auto kernel = few ? k_logits<decltype(t), kLogitsShort> : k_logits<decltype(t), kLogitsLong>;
+            launch(s, dim3(unsigned(a.segments), unsigned(g->rows)), dim3(kLogitsThreads), 0, kernel, a);
         });
-        if (g->argmax) launch(s, dim3(unsigned(g->rows)), dim3(32), 0, k_logits_pick, a.best, a.segments, g->argmax);
+        if (g->argmax) launch_after(s, dim3(unsigned(g->rows)), dim3(32), k_logits_pick, a.best, a.segments, g->argmax);
     });
 }
 

@@ -83,22 +83,46 @@ struct AppendArgs {
     FastDiv by_page;
 };
 
-// One CTA per token: its key and value heads to their page, element by element.
-template <typename T> __global__ void __launch_bounds__(128) k_paged_append(AppendArgs a) {
-    const int token = blockIdx.x;
-    const int slot = a.starts ? slot_of(a.starts, a.slots, token) : token;
-    if (slot < 0) return;
-    const int len = held_rows(a.lengths, slot, a.width, a.page);
-    const int pos = a.starts ? len - a.starts[slot + 1] + token : len - 1;
-    if (pos < 0) return;
-    const int entry = int(a.by_page.div(uint32_t(pos)));
-    const int id = a.table[slot * a.ts + entry];
-    if (id < 0 || id >= a.pages) return;
-    const int row = pos - entry * a.page;
-    for (int e = threadIdx.x; e < a.kv * a.dim; e += blockDim.x) {
-        const int h = e / a.dim, d = e % a.dim;
-        static_cast<T*>(a.k)[id * a.kp + row * a.kr + h * a.kh + d] = static_cast<const T*>(a.nk)[token * a.nkt + h * a.nkh + d];
-        static_cast<T*>(a.v)[id * a.vp + row * a.vr + h * a.vh + d] = static_cast<const T*>(a.nv)[token * a.nvt + h * a.nvh + d];
+// 16-byte words of new rows to their pages, kAppendTokens tokens a CTA: the places of its tokens are looked up once, a thread
+// each, then all threads copy. `vector`: source rows are 16-byte aligned (the pools always are). Bound by HBM, and by the
+// three dependent reads (starts, lengths, table) where there are few tokens.
+constexpr int kAppendTokens = 8;
+template <typename T> __global__ void __launch_bounds__(256) k_paged_append(AppendArgs a, int vector) {
+    __shared__ int64_t places[kAppendTokens][2];
+    const int token0 = blockIdx.x * kAppendTokens;
+    if (threadIdx.x < kAppendTokens) {
+        const int token = token0 + threadIdx.x;
+        int64_t kplace = -1, vplace = -1;
+        const int slot = token >= a.tokens ? -1 : a.starts ? slot_of(a.starts, a.slots, token) : token;
+        if (slot >= 0) {
+            const int len = held_rows(a.lengths, slot, a.width, a.page);
+            const int pos = a.starts ? len - a.starts[slot + 1] + token : len - 1;
+            if (pos >= 0) {
+                const int entry = int(a.by_page.div(uint32_t(pos))), id = a.table[slot * a.ts + entry];
+                if (id >= 0 && id < a.pages) {
+                    kplace = id * a.kp + (pos - entry * a.page) * a.kr;
+                    vplace = id * a.vp + (pos - entry * a.page) * a.vr;
+                }
+            }
+        }
+        places[threadIdx.x][0] = kplace;
+        places[threadIdx.x][1] = vplace;
+    }
+    __syncthreads();
+    constexpr int kPer = 16 / sizeof(T);
+    const int run = a.dim / kPer, words = a.kv * run;  // of a token's keys, or values
+#pragma unroll 4
+    for (int e = threadIdx.x; e < kAppendTokens * 2 * words; e += 256) {
+        const int t = e / (2 * words), rest = e % (2 * words), value = rest >= words, w = rest - value * words;
+        const int h = w / run, d = (w - h * run) * kPer, token = token0 + t;
+        const int64_t place = places[t][value];
+        if (place < 0) continue;
+        const T* from = static_cast<const T*>(value ? a.nv : a.nk) + token * (value ? a.nvt : a.nkt) + h * (value ? a.nvh : a.nkh) + d;
+        T* to = static_cast<T*>(value ? a.v : a.k) + place + h * (value ? a.vh : a.kh) + d;
+        if (vector) *reinterpret_cast<uint4*>(to) = __ldg(reinterpret_cast<const uint4*>(from));
+        else
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) to[i] = from[i];
     }
 }
 

@@ -66,12 +66,11 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
     return v + (warp ? warp_sums[warp - 1] : 0);
 }
 
-// New table rows from the parents', and each page's keeper: the holder with the most rows in it, then the lowest slot.
-__global__ void __launch_bounds__(256) k_pages_gather(StepArgs a) {
-    const int slot = blockIdx.y, m = blockIdx.x * 256 + threadIdx.x;
+// Entry m of a slot's new table row, from its parent's, and the page's keeper: the holder with the most rows in it, then the
+// lowest slot.
+__device__ __forceinline__ void gather_entry(const StepArgs& a, unsigned* keeper, int slot, int m) {
     const SlotStep s = slot_step(a, slot);
     if (m == 0) a.new_lengths[slot] = s.new_rows;
-    if (m >= a.width) return;
     int id = -1;
     const int64_t begin = int64_t(m) * a.page;
     if (begin < s.old_rows) {
@@ -79,25 +78,37 @@ __global__ void __launch_bounds__(256) k_pages_gather(StepArgs a) {
         if (id < 0 || id >= a.pages) id = -1;
         if (id >= 0) {
             const unsigned used = unsigned(min(int64_t(a.page), s.old_rows - begin));
-            atomicMax(&a.keeper[id], used * unsigned(a.slots) + unsigned(a.slots - 1 - slot) + 1u);
+            atomicMax(&keeper[id], used * unsigned(a.slots) + unsigned(a.slots - 1 - slot) + 1u);
         }
     }
     a.new_table[int64_t(slot) * a.width + m] = id;
 }
 
+[[maybe_unused]] static __global__ void __launch_bounds__(256) k_pages_gather(StepArgs a) {
+    const int m = blockIdx.x * 256 + threadIdx.x;
+    if (m < a.width) gather_entry(a, a.keeper, blockIdx.y, m);
+}
+
+// One CTA of 1,024: the numbers of the pages for which pick(p) holds, in ascending order, through put(rank, p). Returns how
+// many there are.
+template <typename Pick, typename Put>
+__device__ __forceinline__ int list_pages(int pages, int* warp_sums, Pick&& pick, Put&& put) {
+    const int per = (pages + 1023) / 1024, p0 = threadIdx.x * per, p1 = min(pages, p0 + per);
+    int mine = 0, total;
+    for (int p = p0; p < p1; ++p) mine += pick(p);
+    int rank = block_scan(mine, warp_sums, &total) - mine;
+    for (int p = p0; p < p1; ++p)
+        if (pick(p)) put(rank++, p);
+    return total;
+}
+
 // One CTA: the list of free pages, then every slot's share of it.
-__global__ void __launch_bounds__(1024) k_pages_assign(StepArgs a) {
+__device__ __forceinline__ void assign_pages(const StepArgs& a, const unsigned* keeper) {
     __shared__ int warp_sums[32];
     __shared__ int s_copies;
     if (threadIdx.x == 0) s_copies = 0;
-    int nfree = 0, total;
-    for (int base = 0; base < a.pages; base += 1024) {
-        const int p = base + threadIdx.x;
-        const int mine = p < a.pages && a.keeper[p] == 0;
-        const int upto = block_scan(mine, warp_sums, &total);
-        if (mine) a.free_list[nfree + upto - 1] = p;
-        nfree += total;
-    }
+    int total;
+    const int nfree = list_pages(a.pages, warp_sums, [&](int p) { return keeper[p] == 0; }, [&](int rank, int p) { a.free_list[rank] = p; });
     __syncthreads();
     int taken = 0;
     for (int base = 0; base < a.slots; base += 1024) {
@@ -112,7 +123,7 @@ __global__ void __launch_bounds__(1024) k_pages_assign(StepArgs a) {
             const int part = s.old_rows % a.page;
             if (part && s.new_rows > s.old_rows) {
                 source = row[held - 1];
-                copy = source >= 0 && a.keeper[source] != unsigned(part) * unsigned(a.slots) + unsigned(a.slots - 1 - slot) + 1u;
+                copy = source >= 0 && keeper[source] != unsigned(part) * unsigned(a.slots) + unsigned(a.slots - 1 - slot) + 1u;
             }
         }
         const int upto = block_scan(copy + fresh, warp_sums, &total);
@@ -141,22 +152,49 @@ __global__ void __launch_bounds__(1024) k_pages_assign(StepArgs a) {
     }
 }
 
-// The first rows of page `source` of every layer's keys and values to page `target`, for each entry of a list in
-// device memory.
-__global__ void __launch_bounds__(256) k_pages_copy(PoolArgs a, const int* list, const int* count) {
-    const int n = *count;
-    for (int64_t item = blockIdx.x; item < int64_t(n) * a.layers * 2; item += gridDim.x) {
-        const int c = int(item / (2 * a.layers)), layer = int(item % (2 * a.layers)) >> 1;
+[[maybe_unused]] static __global__ void __launch_bounds__(1024) k_pages_assign(StepArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" :::);
+    assign_pages(a, a.keeper);
+}
+
+// The whole decision in one CTA, the keepers in shared memory [pages].
+[[maybe_unused]] static __global__ void __launch_bounds__(1024) k_pages_step(StepArgs a) {
+    extern __shared__ unsigned page_marks[];
+    asm volatile("griddepcontrol.launch_dependents;" :::);
+    for (int p = threadIdx.x; p < a.pages; p += 1024) page_marks[p] = 0;
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.slots * a.width; e += 1024) gather_entry(a, page_marks, e / a.width, e % a.width);
+    __syncthreads();
+    assign_pages(a, page_marks);
+}
+
+// The first rows of page `source` of every layer's keys and values to page `target`, for each entry (source, target, rows)
+// of a list in device memory: 16 KB a CTA at a time, four words a thread under way.
+[[maybe_unused]] static __global__ void __launch_bounds__(256) k_pages_copy(PoolArgs a, const int* list, const int* count) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int row_words = a.heads * a.run, part = blockIdx.y;  // 1,024 words of a page
+    const bool plain = a.heads == 1 && a.kr == a.run && a.vr == a.run;  // a page is one run
+    const int64_t total = int64_t(*count) * a.layers * 2;
+    for (int64_t item = blockIdx.x; item < total; item += gridDim.x) {
+        const unsigned c = unsigned(item) / unsigned(2 * a.layers), layer = unsigned(item) % unsigned(2 * a.layers) >> 1;
         const bool value = item & 1;
-        const int64_t source = list[3 * c], target = list[3 * c + 1];
-        const int words = list[3 * c + 2] * a.heads * a.run;
-        uint4* pool = (value ? a.v : a.k) + layer * (value ? a.vl : a.kl);
+        const int words = list[3 * c + 2] * row_words, w0 = part * 1024 + threadIdx.x;
+        if (part * 1024 >= words) continue;
         const int64_t sp = value ? a.vp : a.kp, sr = value ? a.vr : a.kr, sh = value ? a.vh : a.kh;
-        for (int w = threadIdx.x; w < words; w += 256) {
-            const int row = w / (a.heads * a.run), rest = w % (a.heads * a.run);
-            const int64_t off = row * sr + (rest / a.run) * sh + rest % a.run;
-            pool[target * sp + off] = pool[source * sp + off];
+        uint4* pool = (value ? a.v : a.k) + layer * (value ? a.vl : a.kl);
+        const uint4* from = pool + list[3 * c] * sp;
+        uint4* to = pool + list[3 * c + 1] * sp;
+        int64_t off[4];
+        uint4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int w = w0 + i * 256;
+            off[i] = plain ? w : w / row_words * sr + w % row_words / a.run * sh + w % a.run;
+            if (w < words) x[i] = from[off[i]];
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (w0 + i * 256 < words) to[off[i]] = x[i];
     }
 }
 
@@ -165,50 +203,37 @@ struct CompactArgs {
     int64_t ts;
     const int* lengths;
     int *new_table, *info;
-    unsigned* held;    // [pages]
-    int* to;           // [pages] new number of a held page
+    unsigned* held;    // [pages] marks; then 1 + the new number of a held page
     int* copies;       // [pages][3] and the count behind it
     int slots, width, pages, page;
 };
 
-__global__ void __launch_bounds__(256) k_compact_mark(CompactArgs a) {
-    const int slot = blockIdx.y, m = blockIdx.x * 256 + threadIdx.x;
-    if (m >= a.width || int64_t(m) * a.page >= held_rows(a.lengths, slot, a.width, a.page)) return;
+__device__ __forceinline__ int held_entry(const CompactArgs& a, int slot, int m) {  // the page there, or -1
+    if (int64_t(m) * a.page >= held_rows(a.lengths, slot, a.width, a.page)) return -1;
     const int id = a.table[slot * a.ts + m];
-    if (id >= 0 && id < a.pages) a.held[id] = 1;
+    return id >= 0 && id < a.pages ? id : -1;
 }
 
-__global__ void __launch_bounds__(1024) k_compact_plan(CompactArgs a) {
+// One CTA: held[p] becomes 1 + the new number of each held page; the list of moves.
+__device__ __forceinline__ void plan_moves(const CompactArgs& a, unsigned* held) {
     __shared__ int warp_sums[32];
-    int n = 0, total;
-    for (int base = 0; base < a.pages; base += 1024) {
-        const int p = base + threadIdx.x;
-        block_scan(p < a.pages && a.held[p], warp_sums, &total);
-        n += total;
+    int n;
+    {
+        const int per = (a.pages + 1023) / 1024, p0 = threadIdx.x * per, p1 = min(a.pages, p0 + per);
+        int mine = 0;
+        for (int p = p0; p < p1; ++p) mine += held[p] != 0;
+        block_scan(mine, warp_sums, &n);
     }
-    int holes = 0;
-    for (int base = 0; base < n; base += 1024) {
-        const int p = base + threadIdx.x;
-        const int mine = p < n && !a.held[p];
-        const int upto = block_scan(mine, warp_sums, &total);
-        if (mine) a.copies[3 * (holes + upto - 1) + 1] = p;
-        if (p < n && !mine) a.to[p] = p;
-        holes += total;
-    }
+    list_pages(n, warp_sums, [&](int p) { return held[p] == 0; }, [&](int rank, int p) { a.copies[3 * rank + 1] = p; });
     __syncthreads();
-    int moved = 0;
-    for (int base = n; base < a.pages; base += 1024) {
-        const int p = base + threadIdx.x;
-        const int mine = p < a.pages && a.held[p];
-        const int upto = block_scan(mine, warp_sums, &total);
-        if (mine) {
-            int* c = a.copies + 3 * (moved + upto - 1);
-            c[0] = p;
-            c[2] = a.page;
-            a.to[p] = c[1];
-        }
-        moved += total;
-    }
+    const int moved = list_pages(a.pages - n, warp_sums, [&](int p) { return held[n + p] != 0; }, [&](int rank, int p) {
+        a.copies[3 * rank] = n + p;
+        a.copies[3 * rank + 2] = a.page;
+    });
+    __syncthreads();
+    for (int p = threadIdx.x; p < n; p += 1024)
+        if (held[p]) held[p] = p + 1;
+    for (int i = threadIdx.x; i < moved; i += 1024) held[a.copies[3 * i]] = a.copies[3 * i + 1] + 1;
     if (threadIdx.x == 0) {
         a.copies[3 * a.pages] = moved;
         a.info[0] = n;
@@ -216,12 +241,36 @@ __global__ void __launch_bounds__(1024) k_compact_plan(CompactArgs a) {
     }
 }
 
-__global__ void __launch_bounds__(256) k_compact_table(CompactArgs a) {
-    const int slot = blockIdx.y, m = blockIdx.x * 256 + threadIdx.x;
-    if (m >= a.width) return;
-    int id = -1;
-    if (int64_t(m) * a.page < held_rows(a.lengths, slot, a.width, a.page)) id = a.table[slot * a.ts + m];
-    a.new_table[int64_t(slot) * a.width + m] = id >= 0 && id < a.pages ? a.to[id] : -1;
+__device__ __forceinline__ void renumber_entry(const CompactArgs& a, const unsigned* held, int slot, int m) {
+    const int id = held_entry(a, slot, m);
+    a.new_table[int64_t(slot) * a.width + m] = id >= 0 ? int(held[id]) - 1 : -1;
+}
+
+[[maybe_unused]] static __global__ void __launch_bounds__(256) k_compact_mark(CompactArgs a) {
+    const int m = blockIdx.x * 256 + threadIdx.x, id = m < a.width ? held_entry(a, blockIdx.y, m) : -1;
+    if (id >= 0) a.held[id] = 1;
+}
+[[maybe_unused]] static __global__ void __launch_bounds__(1024) k_compact_plan(CompactArgs a) { plan_moves(a, a.held); }
+[[maybe_unused]] static __global__ void __launch_bounds__(256) k_compact_table(CompactArgs a) {
+    const int m = blockIdx.x * 256 + threadIdx.x;
+    asm volatile("griddepcontrol.launch_dependents;" :::);
+    if (m < a.width) renumber_entry(a, a.held, blockIdx.y, m);
+}
+
+// The whole decision in one CTA, the marks in shared memory [pages].
+[[maybe_unused]] static __global__ void __launch_bounds__(1024) k_compact(CompactArgs a) {
+    extern __shared__ unsigned page_marks[];
+    asm volatile("griddepcontrol.launch_dependents;" :::);
+    for (int p = threadIdx.x; p < a.pages; p += 1024) page_marks[p] = 0;
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.slots * a.width; e += 1024) {
+        const int id = held_entry(a, e / a.width, e % a.width);
+        if (id >= 0) page_marks[id] = 1;
+    }
+    __syncthreads();
+    plan_moves(a, page_marks);
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.slots * a.width; e += 1024) renumber_entry(a, page_marks, e / a.width, e % a.width);
 }
 
 }  // namespace cb200

@@ -282,8 +282,9 @@ typedef struct chroma_b200_attention {
  * token that sees nothing gives zeros, and its sink (or -inf) as lse. */
 int chroma_b200_paged_attention(const chroma_b200_pages* pages, const chroma_b200_attention* args, void* stream,
                                 char* err, size_t err_len);
-/* Bytes of workspace that paged_attention wants for these heads and this head_dim on the current device. */
-int64_t chroma_b200_attention_workspace(int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim);
+/* Bytes of workspace that this call wants on the current device (0: none; -1: wrong arguments); its pointers are not
+ * looked at. */
+int64_t chroma_b200_attention_workspace(const chroma_b200_pages* pages, const chroma_b200_attention* args);
 
 /* One step of a set of sequences. Slot s continues slot parents[s] (any slot may be continued by several; -1, or any
  * other number that is no slot, empties s), and counts[s] more rows are reserved for it. Writes the new table
