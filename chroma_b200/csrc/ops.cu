@@ -492,6 +492,7 @@ int chroma_b200_process_logits(const chroma_b200_logits* g, void* stream, char* 
         a.vocab = g->vocab, a.width = g->width, a.biases = g->biases;
         const int64_t size = int64_t(element(g->storage));
         a.vector = aligned16(g->logits) && aligned16(g->out) && (g->rows == 1 || (g->stride * size % 16 == 0 && g->out_stride * size % 16 == 0));
+        a.history_vector = aligned16(g->history) && (g->rows == 1 || g->history_stride % 4 == 0);
         // Long segments once they alone give every SM two CTAs.
         const bool few = int64_t(g->rows) * ((g->vocab + kLogitsLong - 1) / kLogitsLong) < 2 * sm_count();
         const int segment = few ? kLogitsShort : kLogitsLong;

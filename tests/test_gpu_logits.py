@@ -107,6 +107,19 @@ def test_infinities_ties_and_rows_with_nothing_allowed(gpu) -> None:  # type: ig
     assert ids.tolist()[0] == 0 and bool(torch.isneginf(got[:, [100, 5000]]).all())
 
 
+def test_temperatures_divide(gpu) -> None:  # type: ignore[no-untyped-def]
+    # l / temperature is the correctly rounded quotient, bit for bit, of ordinary values and of extreme ones.
+    g = torch.Generator(device="cuda").manual_seed(8)
+    bits = torch.randint(-(2**31), 2**31, (40, 40000), generator=g, device="cuda").to(torch.int32)
+    x = bits.view(torch.float32).clone()
+    x[:20] = torch.randn(20, 40000, generator=g, device="cuda") * 5
+    x[x.isnan()] = 0.0
+    t = torch.rand(40, generator=g, device="cuda") + 0.3
+    t[5], t[6], t[25], t[26] = 1e-20, 3e25, 1e-38, 1e30
+    got = chroma_b200.process_logits(x, temperature=t)
+    assert torch.equal(got, x / t[:, None])
+
+
 def test_biases_add_up_in_list_order(gpu) -> None:  # type: ignore[no-untyped-def]
     x = torch.zeros(1, 300, device="cuda")
     values = torch.tensor([[1e8, 1.0, -1e8, 1.0] * 20], device="cuda")
