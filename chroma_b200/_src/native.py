@@ -154,20 +154,6 @@ def call(name: str, *args: Any) -> None:
         raise _ERRORS.get(status, RuntimeError)(err.value.decode(errors="replace") or name)
 
 
-_local = threading.local()
-
-
-def call_op(name: str, *args: Any) -> None:
-    """``call`` for operators that run every few microseconds: one message buffer per thread."""
-    try:
-        err = _local.err
-    except AttributeError:
-        err = _local.err = ctypes.create_string_buffer(1024)
-    status = getattr(_lib or lib(), name)(*args, err, 1024)
-    if status != OK:
-        raise _ERRORS.get(status, RuntimeError)(err.value.decode(errors="replace") or name)
-
-
 # ---------------------------------------------------------------------------------------------------------
 # Page-locked result arrays.
 

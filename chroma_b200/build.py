@@ -1,7 +1,8 @@
-"""Build step: compile the sm_100a kernels and the C ABI into ``chroma_b200/libchroma_b200.so`` (in-tree).
+"""Build step: compile the sm_100a kernels and the C ABI into ``chroma_b200/libchroma_b200.so`` (in-tree), and the
+binding of the operators on CUDA tensors into ``chroma_b200/_src/_tensors.so``.
 
 nvcc cross-compiles without a GPU. The library links the CUDA runtime statically so it loads wherever the driver
-is present.
+is present. The binding is built against the installed Torch; nothing but those operators needs it.
 """
 
 from __future__ import annotations
@@ -10,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -17,6 +19,8 @@ ROOT = PACKAGE.parent
 SOURCES = [PACKAGE / "csrc" / "runtime.cu", PACKAGE / "csrc" / "graph.cu", PACKAGE / "csrc" / "ops.cu"]
 DEPENDS = sorted((PACKAGE / "csrc").glob("*.cu*")) + [ROOT / "include" / "chroma_b200.h"]
 TARGET = PACKAGE / "libchroma_b200.so"
+TENSORS = PACKAGE / "_src" / "_tensors.so"
+TENSORS_SOURCE = PACKAGE / "csrc" / "tensors.cpp"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -32,22 +36,38 @@ def command(target: Path = TARGET) -> list[str]:
             "-I", str(ROOT / "include"), *map(str, SOURCES), "-o", str(target)]
 
 
-def stale() -> bool:
-    if not TARGET.exists():
+def tensors_command(target: Path = TENSORS) -> list[str]:
+    import torch
+
+    home = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", str(TENSORS_SOURCE), "-o", str(target),
+            "-I", sysconfig.get_paths()["include"], "-isystem", str(home / "include"), "-isystem",
+            str(cuda / "include"), "-L", str(home / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+
+
+def stale(target: Path = TARGET, depends: list[Path] = DEPENDS) -> bool:
+    if not target.exists():
         return True
-    built = TARGET.stat().st_mtime
-    return any(p.stat().st_mtime > built for p in DEPENDS)
+    built = target.stat().st_mtime
+    return any(p.stat().st_mtime > built for p in depends)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    if force or stale():
-        tmp = TARGET.with_suffix(".so.tmp")
-        res = subprocess.run(command(tmp), capture_output=True, text=True)
-        if res.returncode:
-            raise RuntimeError(f"nvcc failed:\n{res.stderr}")
-        if verbose and res.stderr:
-            print(res.stderr, file=sys.stderr)
-        os.replace(tmp, TARGET)
+    jobs = []
+    for target, depends, make in ((TARGET, DEPENDS, command), (TENSORS, [TENSORS_SOURCE, *DEPENDS[-1:]], tensors_command)):
+        if force or stale(target, depends):
+            tmp = target.with_suffix(".so.tmp")
+            args = make(tmp)
+            jobs.append((target, tmp, args[0], subprocess.Popen(args, stderr=subprocess.PIPE, text=True)))
+    for target, tmp, compiler, process in jobs:
+        _, messages = process.communicate()
+        if process.returncode:
+            raise RuntimeError(f"{Path(compiler).name} failed:\n{messages}")
+        if verbose and messages:
+            print(messages, file=sys.stderr)
+        os.replace(tmp, target)
     return TARGET
 
 
