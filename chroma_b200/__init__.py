@@ -38,7 +38,7 @@ def compile_model(model: Any, output: str | Path, *, steps: int, context: int | 
 # Operators on CUDA tensors of the caller (a paged key-value cache, its attention, logits): Torch is imported by the
 # caller, who has the tensors.
 _OPERATORS = {"paged_append": "paged", "paged_attention": "paged", "step_pages": "paged", "compact_pages": "paged",
-              "process_logits": "logits"}
+              "check_operators": "paged", "process_logits": "logits"}
 
 
 def __getattr__(name: str) -> Any:

@@ -112,6 +112,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "chroma_b200_pages_workspace": (ctypes.c_int64, [_I32, _I32]),
     "chroma_b200_process_logits": (ctypes.c_int, [_VP, _VP, _CP, _SZ]),
     "chroma_b200_logits_workspace": (ctypes.c_int64, [_I32, _I32]),
+    "chroma_b200_operators_check": (ctypes.c_int, [_VP, _CP, _SZ]),
 }
 
 EP_HANDLE_BYTES = 64  # CHROMA_B200_EP_HANDLE_BYTES

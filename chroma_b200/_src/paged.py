@@ -14,8 +14,8 @@ sequence (below 0: none); and int32 ``lengths [slots]``, the rows that each hold
 
 Pools may have any strides that are multiples of 16 bytes (a layer of a larger pool, keys and values side by side); a
 head's row is contiguous and a multiple of 16 bytes. Everything is queued on the current stream of the tensors' device;
-nothing waits for the device or reads it from the host. Wrong arguments raise ``ValueError`` (``TypeError`` for what is
-not a tensor).
+nothing waits for the device or reads it from the host (``check_operators`` does). Wrong arguments raise ``ValueError``
+(``TypeError`` for what is not a tensor). The binding is ``chroma_b200/csrc/tensors.cpp``.
 """
 
 from __future__ import annotations
@@ -99,3 +99,11 @@ def compact_pages(table: Tensor, lengths: Tensor, keys: Tensor, values: Tensor) 
     page from n up goes to the i-th free page below n. Returns the new table and ``info`` (int32, on the device):
     [n, pages moved]."""
     return ops.compact_pages(table, lengths, keys, values)
+
+
+def check_operators(device: Any = None) -> None:
+    """Waits for the current stream of ``device`` (the current one unless given), and raises ``RuntimeError`` if since the
+    last check there a kernel of the operators gave up on a bounded wait inside itself: its outputs are incomplete. A program
+    calls it where it synchronises anyway."""
+    with torch.cuda.device(device):
+        nat.call("chroma_b200_operators_check", torch.cuda.current_stream().cuda_stream)

@@ -343,6 +343,19 @@ dim3 table_grid(const chroma_b200_pages& p) { return dim3(unsigned((p.width + 25
 
 extern "C" {
 
+int chroma_b200_operators_check(void* stream, char* err, size_t err_len) {
+    return guarded_op(err, err_len, [&] {
+        unsigned word = 0;
+        unsigned* at = error_word();
+        const auto s = cudaStream_t(stream);
+        check(cudaMemcpyAsync(&word, at, sizeof word, cudaMemcpyDeviceToHost, s), "error word");
+        check(cudaStreamSynchronize(s), "operators");
+        if (!word) return;
+        check(cudaMemsetAsync(at, 0, sizeof word, s), "error word");
+        throw std::runtime_error("a bounded wait inside an operator's kernel timed out; its outputs are incomplete");
+    });
+}
+
 int chroma_b200_paged_append(const chroma_b200_pages* p, const void* new_keys, const void* new_values,
                              const int64_t* new_strides, const int32_t* starts, int32_t tokens, void* stream, char* err,
                              size_t err_len) {

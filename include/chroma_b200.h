@@ -326,6 +326,10 @@ typedef struct chroma_b200_logits {
 int chroma_b200_process_logits(const chroma_b200_logits* args, void* stream, char* err, size_t err_len);
 int64_t chroma_b200_logits_workspace(int32_t rows, int32_t vocab);
 
+/* Waits for `stream` and raises CHROMA_B200_RUNTIME if, since the last check on the current device, a kernel of these
+ * operators gave up on a bounded wait inside itself (its outputs are then incomplete). */
+int chroma_b200_operators_check(void* stream, char* err, size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif
