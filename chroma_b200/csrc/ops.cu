@@ -328,11 +328,13 @@ void copy_pages(const chroma_b200_pages& p, const int* list, const int* count, c
     launch_after(s, dim3(unsigned(columns), unsigned(parts)), dim3(256), k_pages_copy, a, list, count);
 }
 
-// One CTA decides about pages whose marks fit its shared memory and whose table it reads in a few rounds.
-bool one_cta(const chroma_b200_pages& p) { return p.pages <= 48 * 1024 && int64_t(p.slots) * p.width <= 64 * 1024; }
+// One CTA decides about pages and slots that fit its shared memory, and a table that it reads in a few rounds.
+bool one_cta(const chroma_b200_pages& p) {
+    return p.pages <= 32 * 1024 && p.slots <= 4096 && int64_t(p.slots) * p.width <= 64 * 1024;
+}
 
 template <typename K> size_t shared_marks(K kernel, const chroma_b200_pages& p) {
-    const size_t bytes = size_t(p.pages) * 4;
+    const size_t bytes = size_t(p.pages) * 4 + size_t(p.slots) * sizeof(SlotStep);
     if (bytes > 48 * 1024) check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)), "smem attribute");
     return bytes;
 }
@@ -375,10 +377,11 @@ int chroma_b200_paged_append(const chroma_b200_pages* p, const void* new_keys, c
         a.slots = p->slots, a.width = p->width, a.pages = p->pages, a.page = p->page_rows, a.kv = p->kv_heads;
         a.dim = p->head_dim, a.tokens = tokens, a.by_page = FastDiv(uint32_t(p->page_rows));
         const int64_t size = int64_t(element(p->storage));
+        a.by_run = FastDiv(uint32_t(p->head_dim * size / 16));
         int vector = aligned16(new_keys) && aligned16(new_values);
         for (int i = 0; i < 4; ++i) vector = vector && new_strides[i] * size % 16 == 0;
         by_type(p->storage, [&](auto t) {
-            launch(cudaStream_t(stream), dim3(unsigned((tokens + kAppendTokens - 1) / kAppendTokens)), dim3(256), 0, k_paged_append<decltype(t)>, a, vector);
+            launch(cudaStream_t(stream), dim3(unsigned((tokens + kAppendWarps - 1) / kAppendWarps)), dim3(32 * kAppendWarps), 0, k_paged_append<decltype(t)>, a, vector);
         });
     });
 }

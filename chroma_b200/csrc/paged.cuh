@@ -80,49 +80,78 @@ struct AppendArgs {
     const int* lengths;
     const int* starts;
     int slots, width, pages, page, kv, dim, tokens;
-    FastDiv by_page;
+    FastDiv by_page, by_run;        // by_run.d: 16-byte words of a head's row
 };
 
-// 16-byte words of new rows to their pages, kAppendTokens tokens a CTA: the places of its tokens are looked up once, a thread
-// each, then all threads copy. `vector`: source rows are 16-byte aligned (the pools always are). Bound by HBM, and by the
-// three dependent reads (starts, lengths, table) where there are few tokens.
-constexpr int kAppendTokens = 8;
-template <typename T> __global__ void __launch_bounds__(256) k_paged_append(AppendArgs a, int vector) {
-    __shared__ int64_t places[kAppendTokens][2];
-    const int token0 = blockIdx.x * kAppendTokens;
-    if (threadIdx.x < kAppendTokens) {
-        const int token = token0 + threadIdx.x;
-        int64_t kplace = -1, vplace = -1;
-        const int slot = token >= a.tokens ? -1 : a.starts ? slot_of(a.starts, a.slots, token) : token;
-        if (slot >= 0) {
-            const int len = held_rows(a.lengths, slot, a.width, a.page);
-            const int pos = a.starts ? len - a.starts[slot + 1] + token : len - 1;
-            if (pos >= 0) {
-                const int entry = int(a.by_page.div(uint32_t(pos))), id = a.table[slot * a.ts + entry];
-                if (id >= 0 && id < a.pages) {
-                    kplace = id * a.kp + (pos - entry * a.page) * a.kr;
-                    vplace = id * a.vp + (pos - entry * a.page) * a.vr;
-                }
+// New rows to their pages, a warp per token, 16 bytes a lane. The warp's first words are read while its token's place is looked
+// up; up to 256 slots are all compared with the token at once (one read deep), more are searched. `vector`: source rows are
+// 16-byte aligned (the pools always are). Bound by HBM, and by the three dependent reads (starts and lengths, table, then the
+// stores) where there are few tokens.
+constexpr int kAppendWarps = 8;
+template <typename T> __global__ void __launch_bounds__(32 * kAppendWarps) k_paged_append(AppendArgs a, int vector) {
+    constexpr int kPer = 16 / sizeof(T), kAtOnce = 4;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, token = blockIdx.x * kAppendWarps + warp;
+    if (token >= a.tokens) return;
+    const int words = a.kv * int(a.by_run.d), total = 2 * words;  // words of the token's keys, then of its values
+    const T *nk = static_cast<const T*>(a.nk) + token * a.nkt, *nv = static_cast<const T*>(a.nv) + token * a.nvt;
+    const auto split = [&](int e, int& value, int& h, int& d) {
+        value = e >= words;
+        const int w = e - value * words;
+        h = int(a.by_run.div(w));
+        d = (w - h * int(a.by_run.d)) * kPer;
+    };
+    uint4 x[kAtOnce];
+    const auto load = [&](int e0) {
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            int value, h, d;
+            const int e = e0 + 32 * i;
+            split(e, value, h, d);
+            if (e < total) x[i] = __ldg(reinterpret_cast<const uint4*>((value ? nv + h * a.nvh : nk + h * a.nkh) + d));
+        }
+    };
+    if (vector) load(lane);
+    int slot = token, pos = -1;
+    if (a.starts && a.slots <= 256) {
+        int found = -1;
+#pragma unroll 4
+        for (int s = lane; s < a.slots; s += 32) {
+            const int first = a.starts[s], end = a.starts[s + 1], held = held_rows(a.lengths, s, a.width, a.page);
+            if (first <= token && token < end) {
+                found = s;
+                pos = held - end + token;
             }
         }
-        places[threadIdx.x][0] = kplace;
-        places[threadIdx.x][1] = vplace;
+        const unsigned who = __ballot_sync(0xffffffffu, found >= 0);
+        if (!who) return;
+        slot = __shfl_sync(0xffffffffu, found, __ffs(who) - 1);
+        pos = __shfl_sync(0xffffffffu, pos, __ffs(who) - 1);
+    } else {
+        if (a.starts) slot = slot_of(a.starts, a.slots, token);
+        if (slot < 0) return;
+        pos = held_rows(a.lengths, slot, a.width, a.page) - (a.starts ? a.starts[slot + 1] - token : 1);
     }
-    __syncthreads();
-    constexpr int kPer = 16 / sizeof(T);
-    const int run = a.dim / kPer, words = a.kv * run;  // of a token's keys, or values
-#pragma unroll 4
-    for (int e = threadIdx.x; e < kAppendTokens * 2 * words; e += 256) {
-        const int t = e / (2 * words), rest = e % (2 * words), value = rest >= words, w = rest - value * words;
-        const int h = w / run, d = (w - h * run) * kPer, token = token0 + t;
-        const int64_t place = places[t][value];
-        if (place < 0) continue;
-        const T* from = static_cast<const T*>(value ? a.nv : a.nk) + token * (value ? a.nvt : a.nkt) + h * (value ? a.nvh : a.nkh) + d;
-        T* to = static_cast<T*>(value ? a.v : a.k) + place + h * (value ? a.vh : a.kh) + d;
-        if (vector) *reinterpret_cast<uint4*>(to) = __ldg(reinterpret_cast<const uint4*>(from));
-        else
+    if (pos < 0) return;
+    const int entry = int(a.by_page.div(uint32_t(pos))), id = a.table[slot * a.ts + entry];
+    if (id < 0 || id >= a.pages) return;
+    T* k = static_cast<T*>(a.k) + id * a.kp + (pos - entry * a.page) * a.kr;
+    T* v = static_cast<T*>(a.v) + id * a.vp + (pos - entry * a.page) * a.vr;
+    for (int e0 = lane; e0 < total; e0 += 32 * kAtOnce) {
+        if (vector && e0 != lane) load(e0);
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) to[i] = from[i];
+        for (int i = 0; i < kAtOnce; ++i) {
+            int value, h, d;
+            const int e = e0 + 32 * i;
+            split(e, value, h, d);
+            if (e >= total) continue;
+            T* to = (value ? v + h * a.vh : k + h * a.kh) + d;
+            if (vector) *reinterpret_cast<uint4*>(to) = x[i];
+            else {
+                const T* from = (value ? nv + h * a.nvh : nk + h * a.nkh) + d;
+#pragma unroll
+                for (int c = 0; c < kPer; ++c) to[c] = from[c];
+            }
+        }
     }
 }
 

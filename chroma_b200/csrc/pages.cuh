@@ -68,9 +68,7 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
 
 // Entry m of a slot's new table row, from its parent's, and the page's keeper: the holder with the most rows in it, then the
 // lowest slot.
-__device__ __forceinline__ void gather_entry(const StepArgs& a, unsigned* keeper, int slot, int m) {
-    const SlotStep s = slot_step(a, slot);
-    if (m == 0) a.new_lengths[slot] = s.new_rows;
+__device__ __forceinline__ void gather_entry(const StepArgs& a, const SlotStep& s, unsigned* keeper, int slot, int m) {
     int id = -1;
     const int64_t begin = int64_t(m) * a.page;
     if (begin < s.old_rows) {
@@ -86,7 +84,9 @@ __device__ __forceinline__ void gather_entry(const StepArgs& a, unsigned* keeper
 
 [[maybe_unused]] static __global__ void __launch_bounds__(256) k_pages_gather(StepArgs a) {
     const int m = blockIdx.x * 256 + threadIdx.x;
-    if (m < a.width) gather_entry(a, a.keeper, blockIdx.y, m);
+    const SlotStep s = slot_step(a, blockIdx.y);
+    if (m == 0) a.new_lengths[blockIdx.y] = s.new_rows;
+    if (m < a.width) gather_entry(a, s, a.keeper, blockIdx.y, m);
 }
 
 // One CTA of 1,024: the numbers of the pages for which pick(p) holds, in ascending order, through put(rank, p). Returns how
@@ -103,7 +103,7 @@ __device__ __forceinline__ int list_pages(int pages, int* warp_sums, Pick&& pick
 }
 
 // One CTA: the list of free pages, then every slot's share of it.
-__device__ __forceinline__ void assign_pages(const StepArgs& a, const unsigned* keeper) {
+template <typename Slot> __device__ __forceinline__ void assign_pages(const StepArgs& a, const unsigned* keeper, Slot&& slot_at) {
     __shared__ int warp_sums[32];
     __shared__ int s_copies;
     if (threadIdx.x == 0) s_copies = 0;
@@ -117,7 +117,7 @@ __device__ __forceinline__ void assign_pages(const StepArgs& a, const unsigned* 
         int copy = 0, fresh = 0, held = 0, source = -1;
         int* row = a.new_table + int64_t(slot) * a.width;
         if (slot < a.slots) {
-            s = slot_step(a, slot);
+            s = slot_at(slot);
             held = pages_of(s.old_rows, a.page);
             fresh = pages_of(s.new_rows, a.page) - held;
             const int part = s.old_rows % a.page;
@@ -154,18 +154,25 @@ __device__ __forceinline__ void assign_pages(const StepArgs& a, const unsigned* 
 
 [[maybe_unused]] static __global__ void __launch_bounds__(1024) k_pages_assign(StepArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" :::);
-    assign_pages(a, a.keeper);
+    assign_pages(a, a.keeper, [&](int slot) { return slot_step(a, slot); });
 }
 
-// The whole decision in one CTA, the keepers in shared memory [pages].
+// The whole decision in one CTA, in shared memory: the keepers [pages] and what becomes of the slots [slots].
 [[maybe_unused]] static __global__ void __launch_bounds__(1024) k_pages_step(StepArgs a) {
     extern __shared__ unsigned page_marks[];
+    SlotStep* steps = reinterpret_cast<SlotStep*>(page_marks + a.pages);
     asm volatile("griddepcontrol.launch_dependents;" :::);
+    for (int slot = threadIdx.x; slot < a.slots; slot += 1024) {
+        const SlotStep s = slot_step(a, slot);
+        steps[slot] = s;
+        a.new_lengths[slot] = s.new_rows;
+    }
     for (int p = threadIdx.x; p < a.pages; p += 1024) page_marks[p] = 0;
     __syncthreads();
-    for (int e = threadIdx.x; e < a.slots * a.width; e += 1024) gather_entry(a, page_marks, e / a.width, e % a.width);
+#pragma unroll 4
+    for (int e = threadIdx.x; e < a.slots * a.width; e += 1024) gather_entry(a, steps[e / a.width], page_marks, e / a.width, e % a.width);
     __syncthreads();
-    assign_pages(a, page_marks);
+    assign_pages(a, page_marks, [&](int slot) { return steps[slot]; });
 }
 
 // The first rows of page `source` of every layer's keys and values to page `target`, for each entry (source, target, rows)
@@ -263,6 +270,7 @@ __device__ __forceinline__ void renumber_entry(const CompactArgs& a, const unsig
     asm volatile("griddepcontrol.launch_dependents;" :::);
     for (int p = threadIdx.x; p < a.pages; p += 1024) page_marks[p] = 0;
     __syncthreads();
+#pragma unroll 4
     for (int e = threadIdx.x; e < a.slots * a.width; e += 1024) {
         const int id = held_entry(a, e / a.width, e % a.width);
         if (id >= 0) page_marks[id] = 1;
@@ -270,6 +278,7 @@ __device__ __forceinline__ void renumber_entry(const CompactArgs& a, const unsig
     __syncthreads();
     plan_moves(a, page_marks);
     __syncthreads();
+#pragma unroll 4
     for (int e = threadIdx.x; e < a.slots * a.width; e += 1024) renumber_entry(a, page_marks, e / a.width, e % a.width);
 }
 
