@@ -288,7 +288,24 @@ void attention_fp32(const PagedArgs& a, const chroma_b200_attention& g, cudaStre
     else run(std::integral_constant<int, 32>());
 }
 
-template <int H> void prompt_bf16(PagedPromptArgs& p, cudaStream_t s) {
+// How prompts are laid out, and their workspace: partial results of every split of every item.
+struct PromptSpace {
+    int64_t items, parts = 0, bytes = 0;  // items: at least as many as there are
+    int splits = 1;
+    PromptSpace(int tokens, int group, int slots, int kv, int dim, int64_t positions) {
+        items = (int64_t(tokens) * group / 256 + (slots < tokens ? slots : tokens)) * kv;
+        if (items < 1) items = 1;
+        // Fewer items than half the SMs share the SMs out, as long as four key tiles are left to each split.
+        const int64_t most = positions / (4 * kPrTile), share = sm_count() / items;
+        if (share > 1 && most > 1) splits = int(share < most ? share : most);
+        if (splits > 1) {
+            parts = items * splits * 256 * (dim <= 64 ? 64 : 128) * 4;
+            bytes = parts + items * splits * 256 * 8;
+        }
+    }
+};
+
+template <int H> void prompt_bf16(PagedPromptArgs& p, const chroma_b200_attention& g, cudaStream_t s) {
     const PagedArgs& a = p.a;
     CUtensorMap kmap{}, vmap{};
     p.box = 0;
@@ -300,14 +317,22 @@ template <int H> void prompt_bf16(PagedPromptArgs& p, cudaStream_t s) {
     const cuuint64_t strides[2] = {cuuint64_t(a.qh * 2), cuuint64_t(a.qt * 2)};
     const cuuint32_t box[3] = {64, cuuint32_t(a.group), cuuint32_t(kPrTile / (a.group <= kPrTile ? a.group : kPrTile))};
     p.q_box = kPrTile % a.group == 0 && bf16_map(&qmap, a.q, 3, dims, strides, box);
-    const int64_t tiles = int64_t(a.tokens) * a.group / 256 + a.slots;  // at least as many as there are
-    const int64_t items = tiles * a.kv;
-    const int grid = int(items < sm_count() ? items : sm_count());
+    const PromptSpace space(a.tokens, a.group, a.slots, a.kv, a.dim, int64_t(a.width) * a.page);
+    p.splits = space.splits;
+    p.by_splits = FastDiv(uint32_t(p.splits));
+    if (p.splits > 1) {
+        want(g.workspace && g.workspace_bytes >= space.bytes, "workspace too small");
+        p.parts = static_cast<float*>(g.workspace);
+        p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(g.workspace) + space.parts);
+    }
+    const int64_t work = space.items * p.splits;
+    const int grid = int(work < sm_count() ? work : sm_count());
     check(cudaFuncSetAttribute(k_paged_prompt<H>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<H>::kSmem), "smem attribute");
     launch(s, dim3(unsigned(grid)), dim3(kPrThreads), PromptShape<H>::kSmem, k_paged_prompt<H>, p, qmap, kmap, vmap);
+    if (p.splits > 1) launch_after(s, dim3(unsigned(space.items * 8)), dim3(256), k_prompt_join<H>, p);
 }
 
-void prompt(const PagedArgs& a, int storage, cudaStream_t s) {
+void prompt(const PagedArgs& a, const chroma_b200_attention& g, int storage, cudaStream_t s) {
     PagedPromptArgs p{};
     p.a = a;
     p.by_group = FastDiv(uint32_t(a.group));
@@ -316,8 +341,8 @@ void prompt(const PagedArgs& a, int storage, cudaStream_t s) {
     const int64_t size = int64_t(element(storage));
     p.q_vector = aligned16(a.q) && a.qt * size % 16 == 0 && a.qh * size % 16 == 0;
     p.out_vector = aligned16(a.out) && a.ot * size % 16 == 0 && a.oh * size % 16 == 0;
-    if (a.dim <= 64) prompt_bf16<1>(p, s);
-    else prompt_bf16<2>(p, s);
+    if (a.dim <= 64) prompt_bf16<1>(p, g, s);
+    else prompt_bf16<2>(p, g, s);
 }
 
 // `list` and `count` as the launch before leaves them on the device.
@@ -389,6 +414,8 @@ int chroma_b200_paged_append(const chroma_b200_pages* p, const void* new_keys, c
 int64_t chroma_b200_attention_workspace(const chroma_b200_pages* p, const chroma_b200_attention* g) {
     if (!p || !g || g->heads <= 0 || p->kv_heads <= 0 || g->heads % p->kv_heads || p->head_dim <= 0) return -1;
     try {
+        if (g->starts && p->storage == CHROMA_B200_BF16)
+            return PromptSpace(g->tokens, g->heads / p->kv_heads, p->slots, p->kv_heads, p->head_dim, int64_t(p->width) * p->page_rows).bytes;
         const DecodeSpace space(g->heads, p->kv_heads, p->head_dim, p->storage);
         return space.whole(p->slots, p->kv_heads, int64_t(p->width) * p->page_rows, g->starts) ? 0 : space.bytes;
     } catch (...) {
@@ -421,7 +448,7 @@ int chroma_b200_paged_attention(const chroma_b200_pages* p, const chroma_b200_at
         a.window = g->window, a.first = g->first, a.scale_log2 = g->scale * kLog2e;
         const auto s = cudaStream_t(stream);
         if (p->storage == CHROMA_B200_FP32) attention_fp32(a, *g, s);
-        else if (g->starts) prompt(a, p->storage, s);
+        else if (g->starts) prompt(a, *g, p->storage, s);
         else decode(a, *g, p->storage, s);
     });
 }

@@ -31,6 +31,9 @@
 // not be finite. Positions that some rows of a tile see and others do not meet the others with weight 0, which is no
 // protection against infinities: a row whose result is not finite is computed again, key by key.
 //
+// Where there are few items (a short chunk after a long cache), the keys of each are split over several CTAs, which leave
+// fp32 partial results for k_prompt_join.
+//
 // All waits are bounded (tma.cuh).
 #pragma once
 
@@ -98,6 +101,10 @@ struct PagedPromptArgs {
     int box;                 // rows of a TMA box; 0: row by row
     int q_vector, out_vector;  // rows are 16-byte aligned
     int q_box;               // Q tiles come as one TMA box: `group` heads of 128 / group tokens
+    int splits;              // of the keys of an item, where there are few items
+    FastDiv by_splits;
+    float* parts;            // [items][splits][256 rows][64 H]: what the splits of a row come to, unless there is one
+    float2* part_ml;         // [items][splits][256 rows]: maximum (log2 domain) and sum
     unsigned* error;
 };
 
@@ -111,9 +118,10 @@ template <int H> struct PromptShape {
 // A work item: 256 rows of one key-value head of one slot, and the key tiles that they see.
 struct PromptItem {
     int slot, kvh, row0, rows, token0, pos0;  // first row; rows of the slot; first token; its position
-    int tiles, pre, main0;                    // key tiles [0, pre), then from main0 on
+    int tiles, skip, pre, main0;              // key tiles of the split, after `skip`: of [0, pre), then from main0 on
     int active;                               // tiles of rows: 1 or 2
-    __device__ __forceinline__ int key0(int t) const { return (t < pre ? t : main0 + t - pre) * kPrTile; }
+    int64_t part;                             // number of this split's first row
+    __device__ __forceinline__ int key0(int t) const { return (skip + t < pre ? skip + t : main0 + skip + t - pre) * kPrTile; }
 };
 
 // The items of a CTA in turn: blockIdx.x, + gridDim.x (backwards every other round, which evens out their sizes), ...
@@ -125,10 +133,21 @@ struct PromptCursor {
         return max(0, t1 - t0) * a.group;
     }
     __device__ __forceinline__ bool next(const PagedPromptArgs& p, int total, PromptItem& w) {
-        const PagedArgs& a = p.a;
         const unsigned i = unsigned(round) * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         ++round;
-        if (i >= unsigned(total) * unsigned(a.kv)) return false;
+        if (i >= unsigned(total) * unsigned(p.a.kv) * unsigned(p.splits)) return false;
+        find(p, p.splits == 1 ? i : p.by_splits.div(i), w);
+        if (p.splits > 1) {
+            const int z = int(i - p.by_splits.div(i) * unsigned(p.splits)), all = w.tiles;
+            w.skip = int(int64_t(all) * z / p.splits);
+            w.tiles = int(int64_t(all) * (z + 1) / p.splits) - w.skip;
+            w.part = int64_t(i) * 256;
+        }
+        return true;
+    }
+    // Item i of all (a later one than the last).
+    __device__ __forceinline__ void find(const PagedPromptArgs& p, unsigned i, PromptItem& w) {
+        const PagedArgs& a = p.a;
         const int tile = int(p.by_kv.div(i));
         w.kvh = int(i) - tile * a.kv;
         int rows = rows_of(a, slot), n = (rows + 255) / 256;
@@ -149,7 +168,8 @@ struct PromptCursor {
         w.pre = (min(a.first, low) + kPrTile - 1) / kPrTile;
         w.main0 = max(low / kPrTile, w.pre);
         w.tiles = last < 0 ? 0 : w.pre + max(0, last / kPrTile - w.main0 + 1);
-        return true;
+        w.skip = 0;
+        w.part = 0;
     }
 };
 
@@ -230,6 +250,7 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap
     constexpr bool kOwnP = H == 1;
     constexpr int kStages = Shape::kStages, D = 64 * H, kO = 512 - 2 * D;
     extern __shared__ uint8_t pr_raw[];
+    asm volatile("griddepcontrol.launch_dependents;" :::);
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pr_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* Qs = sm;                           // [2][H][128][64]
     uint8_t* KV = Qs + 2 * Shape::kTile;        // stage s: K at s * kStage, V kTile behind it
@@ -565,6 +586,24 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap
             }
             if (abort_flag) break;
             // ---- the item's end
+            if (p.splits > 1) {
+                const int64_t at = w.part + k * kPrTile + r;
+                if (w.tiles) {
+                    if (!mbar_wait(&o_done[k], unsigned((kOwnP ? uses - 1 : ends++) & 1), p.error)) abort_flag = 1;
+                    if (abort_flag) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        float ov[32];
+                        tmem_load32(tO + c * 32, ov);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(p.parts + at * D + c * 32 + e) = make_float4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+                    }
+                }
+                p.part_ml[at] = make_float2(m_run, l_run);
+                tc_fence_before();
+                continue;
+            }
             bool again = false;
             const float top = fmaxf(m_run, sink);
             const float c0 = m_run == -INFINITY ? (l_run == 0.f ? 0.f : 1.f) : fast_exp2(m_run - top);
@@ -617,6 +656,53 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap
     if (warp == 8) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the splits of every row, in their order: a warp per row, 32 rows of an item a CTA. A row whose sum is not finite is
+// computed again.
+template <int H> __global__ void __launch_bounds__(256) k_prompt_join(const PagedPromptArgs p) {
+    constexpr int D = 64 * H;
+    __shared__ int s_total;
+    const PagedArgs& a = p.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) s_total = 0;
+    __syncthreads();
+    int mine = 0;
+    for (int s = threadIdx.x; s < a.slots; s += 256) mine += (PromptCursor::rows_of(a, s) + 255) / 256;
+    if (mine) atomicAdd(&s_total, mine);
+    __syncthreads();
+    const unsigned i = blockIdx.x >> 3;
+    if (i >= unsigned(s_total) * unsigned(a.kv)) return;
+    PromptCursor cursor(a);
+    PromptItem w;
+    cursor.find(p, i, w);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int r = (blockIdx.x & 7) * 32 + warp; r < ((blockIdx.x & 7) + 1) * 32; r += 8) {
+        const int row = w.row0 + r, number = int(p.by_group.div(row));
+        if (row >= w.rows) break;
+        const int token = w.token0 + number, head = w.kvh * a.group + row - number * a.group;
+        const auto part = [&](int z) { return (int64_t(i) * p.splits + z) * 256 + r; };
+        float top = -INFINITY, sum = 0.f, x[D / 32] = {};
+        for (int z = lane; z < p.splits; z += 32) top = fmaxf(top, p.part_ml[part(z)].x);
+        top = warp_max(top);
+        for (int z = 0; z < p.splits; ++z) {
+            const float2 ml = p.part_ml[part(z)];
+            const float weight = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - top);
+            if (weight == 0.f) continue;
+            sum += ml.y * weight;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) x[c] += p.parts[part(z) * D + c * 32 + lane] * weight;
+        }
+        float check = sum * 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) check = fmaf(x[c], 0.f, check);
+        float o[4];
+        if (__any_sync(0xffffffffu, check != 0.f)) attend_row<__nv_bfloat16>(a, token, head, w.slot, w.pos0 + number, top, sum, o);
+        else
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[c] = c < D / 32 ? x[c] : 0.f;
+        finish_row<__nv_bfloat16>(a, token, head, top, sum, o);
     }
 }
 

@@ -155,6 +155,27 @@ def test_short_chunk_after_a_long_cache(gpu, dtype) -> None:  # type: ignore[no-
     check(got, want, dtype=dtype, dim=64, lse=logs)
 
 
+@pytest.mark.parametrize("heads,kv,dim,page,window,first,sinks", [
+    (8, 1, 64, 16, 0, 0, True), (8, 2, 128, 48, 0, 0, False), (6, 2, 80, 5, 3000, 300, True), (16, 1, 64, 64, 200, 0, False),
+])
+def test_split_prompts(gpu, heads, kv, dim, page, window, first, sinks) -> None:  # type: ignore[no-untyped-def]
+    # Few rows and many keys: the keys are split. Slots without new rows, with nothing held before, and with nothing to see.
+    new, prior = [5, 0, 40, 1], [7001, 300, 2500, 0]
+    k, v, table, n = cache([a + b for a, b in zip(new, prior)], dtype=B16, kv=kv, dim=dim, page=page)
+    starts = torch.tensor(np.concatenate([[0], np.cumsum(new)]), dtype=torch.int32).cuda()
+    q = queries(sum(new), heads, dim, B16)
+    s = sink_values(heads, F32) if sinks else None
+    n[3] = 0  # a token that is at no position
+    want = ref.attention(q, k, v, table, n, starts, scale=dim**-0.5, window=window, first=first, sinks=s)
+    got, logs = chroma_b200.paged_attention(q, k, v, table, n, starts, window=window, first=first, sinks=s, lse=True)
+    check(got, want, dtype=B16, dim=dim, lse=logs)
+    assert torch.equal(chroma_b200.paged_attention(q, k, v, table, n, starts, window=window, first=first, sinks=s), got)
+    # a value that is not finite where only the later of a tile's tokens see it
+    k[table[2, 2520 // page].item(), 2520 % page] = float("nan")
+    again = chroma_b200.paged_attention(q, k, v, table, n, starts, window=window, first=first, sinks=s)
+    assert torch.equal(again[:25], got[:25]) and bool(again[25].isnan().any())
+
+
 @pytest.mark.parametrize("dtype,heads,kv,dim", [(F32, 4, 2, 16), (B16, 8, 2, 64), (B16, 4, 1, 128)])
 def test_non_finite_rows_reach_only_those_who_see_them(gpu, dtype, heads, kv, dim) -> None:  # type: ignore[no-untyped-def]
     new, prior, page = 150, 20, 16
