@@ -243,7 +243,7 @@ __device__ __forceinline__ uint32_t bits_from_to(int lo, int hi) {  // bits lo..
 
 template <int H>
 __global__ void __launch_bounds__(kPrThreads, 1)
-k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                const __grid_constant__ CUtensorMap vmap) {
     using Shape = PromptShape<H>;
     // TMEM columns: S of the two tiles; P of each over its S (H = 2) or in 64 columns of its own (H = 1); O.
@@ -661,7 +661,7 @@ k_paged_prompt(const PagedPromptArgs p, const __grid_constant__ CUtensorMap qmap
 
 // Joins the splits of every row, in their order: a warp per row, 32 rows of an item a CTA. A row whose sum is not finite is
 // computed again.
-template <int H> __global__ void __launch_bounds__(256) k_prompt_join(const PagedPromptArgs p) {
+template <int H> __global__ void __launch_bounds__(256) k_prompt_join(const __grid_constant__ PagedPromptArgs p) {
     constexpr int D = 64 * H;
     __shared__ int s_total;
     const PagedArgs& a = p.a;
