@@ -4,8 +4,8 @@
 // A row is one query head of one token; the rows of a key-value head are packed, token after token with its `group`
 // query heads side by side, so that a tile of 128 rows shares every key even where a chunk has few tokens. A work item
 // is 256 consecutive rows (two tiles) of one key-value head of one sequence, against key tiles of 128 positions. The
-// grid is persistent, one CTA per SM; items are taken from the last rows of the last sequence backwards (the most keys
-// first), the key-value heads of the same rows side by side. 12 warps:
+// grid is persistent, one CTA per SM; items with the most keys before them come first, the key-value heads of the same rows
+// side by side. 12 warps:
 //   warps 0-3, 4-7  the online softmax of tile 0, 1, one row per thread (TMEM lane = row): the row of S (128 columns)
 //                   from TMEM at once, P = 2^(s - m) back over its first 64 columns as bf16 pairs; at the item's end
 //                   O / l to global memory
@@ -45,6 +45,7 @@ namespace cb200 {
 
 constexpr int kPrThreads = 384, kPrTile = 128;
 // Registers of a softmax thread and of the others, out of the 3 x 168 that three warpgroups are launched with.
+constexpr int kPrSorted = 1024, kPrSortedSlots = 64;  // tiles, slots
 constexpr int kPrSoftmaxRegs = 216, kPrOtherRegs = 72;
 
 // The products are issued by one elected thread of a converged warp: everything they need is the same in all lanes, so it
@@ -124,10 +125,17 @@ struct PromptItem {
     __device__ __forceinline__ int key0(int t) const { return (skip + t < pre ? skip + t : main0 + skip + t - pre) * kPrTile; }
 };
 
+__device__ __forceinline__ uint32_t* prompt_order() {
+    __shared__ uint32_t order[kPrSorted];
+    return order;
+}
+
 // The items of a CTA in turn: blockIdx.x, + gridDim.x (backwards every other round, which evens out their sizes), ...
 struct PromptCursor {
     int slot, before, round;  // tiles of the slots after `slot`
-    __device__ __forceinline__ explicit PromptCursor(const PagedArgs& a) : slot(a.slots - 1), before(0), round(0) {}
+    bool sorted;              // or prompt_order() has slot << 16 | tile of each place
+    __device__ __forceinline__ explicit PromptCursor(const PagedArgs& a, bool in_order = false)
+        : slot(a.slots - 1), before(0), round(0), sorted(in_order) {}
     static __device__ __forceinline__ int rows_of(const PagedArgs& a, int s) {
         const int t0 = min(max(a.starts[s], 0), a.tokens), t1 = min(max(a.starts[s + 1], 0), a.tokens);
         return max(0, t1 - t0) * a.group;
@@ -150,16 +158,25 @@ struct PromptCursor {
         const PagedArgs& a = p.a;
         const int tile = int(p.by_kv.div(i));
         w.kvh = int(i) - tile * a.kv;
-        int rows = rows_of(a, slot), n = (rows + 255) / 256;
-        while (tile >= before + n) {
-            before += n;
-            --slot;
+        int rows;
+        if (sorted) {
+            const uint32_t place = prompt_order()[tile];
+            slot = int(place >> 16);
             rows = rows_of(a, slot);
-            n = (rows + 255) / 256;
+            w.row0 = int(place & 0xffff) * 256;
+        } else {
+            rows = rows_of(a, slot);
+            int n = (rows + 255) / 256;
+            while (tile >= before + n) {
+                before += n;
+                --slot;
+                rows = rows_of(a, slot);
+                n = (rows + 255) / 256;
+            }
+            w.row0 = (n - 1 - (tile - before)) * 256;
         }
         w.slot = slot;
         w.rows = rows;
-        w.row0 = (n - 1 - (tile - before)) * 256;
         w.token0 = min(max(a.starts[slot], 0), a.tokens);
         w.pos0 = held_rows(a.lengths, slot, a.width, a.page) - rows / a.group;
         w.active = w.row0 + kPrTile < rows ? 2 : 1;
@@ -257,7 +274,7 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
     uint32_t* gone = reinterpret_cast<uint32_t*>(KV + kStages * Shape::kStage);  // [kStages][4]
     __shared__ uint64_t q_full[2], q_empty[2], kv_full[kStages], kv_empty[kStages], s_full[2], s_free[2], p_full[2], o_done[2];
     __shared__ uint32_t tmem_base;
-    __shared__ int s_total;
+    __shared__ int s_total, tile_counts[kPrSortedSlots];
     __shared__ volatile int abort_flag;
     const PagedArgs& a = p.a;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -294,7 +311,21 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
     __syncthreads();
     const int total = s_total;
     const uint32_t tmem = tmem_base;
-    PromptCursor cursor(a);
+    // With few sequences their tiles are put in order, the later (with more keys before them) first, whatever the sequence:
+    // four prompts of 2,048 tokens are then within 1% of an even load, against 10% in the order of the sequences.
+    const bool sorted = p.splits == 1 && total <= kPrSorted && a.slots <= kPrSortedSlots;
+    if (sorted) {
+        for (int s = threadIdx.x; s < a.slots; s += kPrThreads) tile_counts[s] = (PromptCursor::rows_of(a, s) + 255) / 256;
+        __syncthreads();
+        for (int e = threadIdx.x; e < total; e += kPrThreads) {
+            int slot = 0, tile = e, place = 0;
+            while (tile >= tile_counts[slot]) tile -= tile_counts[slot++];
+            for (int s = 0; s < a.slots; ++s) place += max(0, tile_counts[s] - 1 - tile) + (s < slot && tile_counts[s] > tile);
+            prompt_order()[place] = uint32_t(slot) << 16 | uint32_t(tile);
+        }
+        __syncthreads();
+    }
+    PromptCursor cursor(a, sorted);
     PromptItem w;
 
     if (warp >= 8) {
