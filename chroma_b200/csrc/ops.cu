@@ -355,11 +355,11 @@ void copy_pages(const chroma_b200_pages& p, const int* list, const int* count, c
 
 // One CTA decides about pages and slots that fit its shared memory, and a table that it reads in a few rounds.
 bool one_cta(const chroma_b200_pages& p) {
-    return p.pages <= 32 * 1024 && p.slots <= 4096 && int64_t(p.slots) * p.width <= 64 * 1024;
+    return p.pages <= 32 * 1024 && p.slots <= 1024 && int64_t(p.slots) * p.width <= 64 * 1024;
 }
 
 template <typename K> size_t shared_marks(K kernel, const chroma_b200_pages& p) {
-    const size_t bytes = size_t(p.pages) * 4 + size_t(p.slots) * sizeof(SlotStep);
+    const size_t bytes = size_t(p.pages) * 4 + size_t(p.slots) * sizeof(SlotStep) + size_t(p.pages) * 2;
     if (bytes > 48 * 1024) check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)), "smem attribute");
     return bytes;
 }
@@ -454,7 +454,7 @@ int chroma_b200_paged_attention(const chroma_b200_pages* p, const chroma_b200_at
 }
 
 int64_t chroma_b200_pages_workspace(int32_t pages, int32_t slots) {
-    return pages < 0 || slots < 0 ? -1 : (4 * int64_t(pages) + 3 * int64_t(slots) + 4) * 4;
+    return pages < 0 || slots < 0 ? -1 : (5 * int64_t(pages) + 3 * int64_t(slots) + 4) * 4;
 }
 
 int chroma_b200_step_pages(const chroma_b200_pages* p, const int32_t* parents, const int32_t* counts, int32_t* new_table,
@@ -497,6 +497,7 @@ int chroma_b200_compact_pages(const chroma_b200_pages* p, int32_t* new_table, in
         a.new_table = new_table, a.info = info;
         a.held = static_cast<unsigned*>(workspace);
         a.copies = static_cast<int*>(workspace) + p->pages;
+        a.holes = a.copies + 3 * p->pages + 1;
         a.slots = p->slots, a.width = p->width, a.pages = p->pages, a.page = p->page_rows;
         if (one_cta(*p)) launch(s, dim3(1), dim3(1024), shared_marks(k_compact, *p), k_compact, a);
         else {

@@ -103,12 +103,13 @@ __device__ __forceinline__ int list_pages(int pages, int* warp_sums, Pick&& pick
 }
 
 // One CTA: the list of free pages, then every slot's share of it.
-template <typename Slot> __device__ __forceinline__ void assign_pages(const StepArgs& a, const unsigned* keeper, Slot&& slot_at) {
+template <typename List, typename Slot>
+__device__ __forceinline__ void assign_pages(const StepArgs& a, const unsigned* keeper, List* free_list, Slot&& slot_at) {
     __shared__ int warp_sums[32];
     __shared__ int s_copies;
     if (threadIdx.x == 0) s_copies = 0;
     int total;
-    const int nfree = list_pages(a.pages, warp_sums, [&](int p) { return keeper[p] == 0; }, [&](int rank, int p) { a.free_list[rank] = p; });
+    const int nfree = list_pages(a.pages, warp_sums, [&](int p) { return keeper[p] == 0; }, [&](int rank, int p) { free_list[rank] = List(p); });
     __syncthreads();
     int taken = 0;
     for (int base = 0; base < a.slots; base += 1024) {
@@ -129,7 +130,7 @@ template <typename Slot> __device__ __forceinline__ void assign_pages(const Step
         const int upto = block_scan(copy + fresh, warp_sums, &total);
         int at = taken + upto - copy - fresh;
         if (copy) {
-            const int target = at < nfree ? a.free_list[at] : -1;
+            const int target = at < nfree ? int(free_list[at]) : -1;
             ++at;
             row[held - 1] = target;
             int* c = a.copies + 3 * atomicAdd(&s_copies, 1);
@@ -137,7 +138,7 @@ template <typename Slot> __device__ __forceinline__ void assign_pages(const Step
             c[1] = target;
             c[2] = s.old_rows % a.page;
         }
-        for (int j = 0; j < fresh; ++j, ++at) row[held + j] = at < nfree ? a.free_list[at] : -1;
+        for (int j = 0; j < fresh; ++j, ++at) row[held + j] = at < nfree ? int(free_list[at]) : -1;
         taken += total;
     }
     __syncthreads();
@@ -154,10 +155,10 @@ template <typename Slot> __device__ __forceinline__ void assign_pages(const Step
 
 [[maybe_unused]] static __global__ void __launch_bounds__(1024) k_pages_assign(StepArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" :::);
-    assign_pages(a, a.keeper, [&](int slot) { return slot_step(a, slot); });
+    assign_pages(a, a.keeper, a.free_list, [&](int slot) { return slot_step(a, slot); });
 }
 
-// The whole decision in one CTA, in shared memory: the keepers [pages] and what becomes of the slots [slots].
+// The whole decision in one CTA, in shared memory: the keepers [pages], what becomes of the slots [slots], the free list.
 [[maybe_unused]] static __global__ void __launch_bounds__(1024) k_pages_step(StepArgs a) {
     extern __shared__ unsigned page_marks[];
     SlotStep* steps = reinterpret_cast<SlotStep*>(page_marks + a.pages);
@@ -172,7 +173,7 @@ template <typename Slot> __device__ __forceinline__ void assign_pages(const Step
 #pragma unroll 4
     for (int e = threadIdx.x; e < a.slots * a.width; e += 1024) gather_entry(a, steps[e / a.width], page_marks, e / a.width, e % a.width);
     __syncthreads();
-    assign_pages(a, page_marks, [&](int slot) { return steps[slot]; });
+    assign_pages(a, page_marks, reinterpret_cast<uint16_t*>(steps + a.slots), [&](int slot) { return steps[slot]; });
 }
 
 // The first rows of page `source` of every layer's keys and values to page `target`, for each entry (source, target, rows)
@@ -212,6 +213,7 @@ struct CompactArgs {
     int *new_table, *info;
     unsigned* held;    // [pages] marks; then 1 + the new number of a held page
     int* copies;       // [pages][3] and the count behind it
+    int* holes;        // [pages]
     int slots, width, pages, page;
 };
 
@@ -221,8 +223,8 @@ __device__ __forceinline__ int held_entry(const CompactArgs& a, int slot, int m)
     return id >= 0 && id < a.pages ? id : -1;
 }
 
-// One CTA: held[p] becomes 1 + the new number of each held page; the list of moves.
-__device__ __forceinline__ void plan_moves(const CompactArgs& a, unsigned* held) {
+// One CTA: held[p] becomes 1 + the new number of each held page; the list of moves. `holes` [pages]: scratch.
+template <typename List> __device__ __forceinline__ void plan_moves(const CompactArgs& a, unsigned* held, List* holes) {
     __shared__ int warp_sums[32];
     int n;
     {
@@ -231,16 +233,17 @@ __device__ __forceinline__ void plan_moves(const CompactArgs& a, unsigned* held)
         for (int p = p0; p < p1; ++p) mine += held[p] != 0;
         block_scan(mine, warp_sums, &n);
     }
-    list_pages(n, warp_sums, [&](int p) { return held[p] == 0; }, [&](int rank, int p) { a.copies[3 * rank + 1] = p; });
+    list_pages(n, warp_sums, [&](int p) { return held[p] == 0; }, [&](int rank, int p) { holes[rank] = List(p); });
     __syncthreads();
     const int moved = list_pages(a.pages - n, warp_sums, [&](int p) { return held[n + p] != 0; }, [&](int rank, int p) {
+        const int to = int(holes[rank]);
         a.copies[3 * rank] = n + p;
+        a.copies[3 * rank + 1] = to;
         a.copies[3 * rank + 2] = a.page;
+        held[n + p] = unsigned(to) + 1;
     });
-    __syncthreads();
     for (int p = threadIdx.x; p < n; p += 1024)
         if (held[p]) held[p] = p + 1;
-    for (int i = threadIdx.x; i < moved; i += 1024) held[a.copies[3 * i]] = a.copies[3 * i + 1] + 1;
     if (threadIdx.x == 0) {
         a.copies[3 * a.pages] = moved;
         a.info[0] = n;
@@ -257,29 +260,44 @@ __device__ __forceinline__ void renumber_entry(const CompactArgs& a, const unsig
     const int m = blockIdx.x * 256 + threadIdx.x, id = m < a.width ? held_entry(a, blockIdx.y, m) : -1;
     if (id >= 0) a.held[id] = 1;
 }
-[[maybe_unused]] static __global__ void __launch_bounds__(1024) k_compact_plan(CompactArgs a) { plan_moves(a, a.held); }
+[[maybe_unused]] static __global__ void __launch_bounds__(1024) k_compact_plan(CompactArgs a) { plan_moves(a, a.held, a.holes); }
 [[maybe_unused]] static __global__ void __launch_bounds__(256) k_compact_table(CompactArgs a) {
     const int m = blockIdx.x * 256 + threadIdx.x;
     asm volatile("griddepcontrol.launch_dependents;" :::);
     if (m < a.width) renumber_entry(a, a.held, blockIdx.y, m);
 }
 
-// The whole decision in one CTA, the marks in shared memory [pages].
+// The whole decision in one CTA, in shared memory: the marks [pages], the holes [pages]. A thread's first entries stay in
+// registers from the marking to the renumbering.
 [[maybe_unused]] static __global__ void __launch_bounds__(1024) k_compact(CompactArgs a) {
     extern __shared__ unsigned page_marks[];
+    constexpr int kKept = 4;
     asm volatile("griddepcontrol.launch_dependents;" :::);
+    int ids[kKept];
+    const int entries = a.slots * a.width;
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) {
+        const int e = threadIdx.x + i * 1024;
+        ids[i] = e < entries ? held_entry(a, e / a.width, e % a.width) : -1;
+    }
     for (int p = threadIdx.x; p < a.pages; p += 1024) page_marks[p] = 0;
     __syncthreads();
-#pragma unroll 4
-    for (int e = threadIdx.x; e < a.slots * a.width; e += 1024) {
+#pragma unroll
+    for (int i = 0; i < kKept; ++i)
+        if (ids[i] >= 0) page_marks[ids[i]] = 1;
+    for (int e = threadIdx.x + kKept * 1024; e < entries; e += 1024) {
         const int id = held_entry(a, e / a.width, e % a.width);
         if (id >= 0) page_marks[id] = 1;
     }
     __syncthreads();
-    plan_moves(a, page_marks);
+    plan_moves(a, page_marks, reinterpret_cast<uint16_t*>(page_marks + a.pages));
     __syncthreads();
-#pragma unroll 4
-    for (int e = threadIdx.x; e < a.slots * a.width; e += 1024) renumber_entry(a, page_marks, e / a.width, e % a.width);
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) {
+        const int e = threadIdx.x + i * 1024;
+        if (e < entries) a.new_table[e] = ids[i] >= 0 ? int(page_marks[ids[i]]) - 1 : -1;
+    }
+    for (int e = threadIdx.x + kKept * 1024; e < entries; e += 1024) renumber_entry(a, page_marks, e / a.width, e % a.width);
 }
 
 }  // namespace cb200
