@@ -277,7 +277,9 @@ void attention_fp32(const PagedArgs& a, const chroma_b200_attention& g, cudaStre
     if (!p.whole) space.place(p, g);
     const auto run = [&](auto words) {
         constexpr int W = decltype(words)::value, DP = W * 4 < 32 ? 32 : W * 4;
-        launch(s, dim3(unsigned(blocks)), dim3(32 * kF32Warps), 0, k_paged_fp32<W>, p, per_item);
+        constexpr int smem = sizeof(F32Space<W>);
+        if (smem > 48 * 1024) check(cudaFuncSetAttribute(k_paged_fp32<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "smem attribute");
+        launch(s, dim3(unsigned(blocks)), dim3(32 * kF32Warps), smem, k_paged_fp32<W>, p, per_item);
         if (p.whole) return;
         if (a.slots >= blocks / lines / 4) launch_after(s, dim3(unsigned(blocks), 1), dim3(256), k_paged_join<float, DP, true>, p, kF32Rows);
         else launch_after(s, dim3(unsigned(blocks), kF32Rows), dim3(256), k_paged_join<float, DP, false>, p, kF32Rows);
