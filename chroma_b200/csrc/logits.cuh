@@ -5,7 +5,13 @@
 // biases of its segment in list order, and passes over the logits once, 16 bytes a thread at a time. No table of counts is
 // kept between calls. The arithmetic is rounded operation by operation (no fused multiply-add), so that results do not
 // depend on how the compiler groups it, and equal logits stay equal. The best of each segment is left for a second, small
-// launch. Bound by HBM where there are many rows; a single row by the latency of its few dependent reads.
+// launch.
+//
+// Bound by latency: each CTA's chain of row length, history, table, logits, best of the segment is longer than its
+// share of the stream. 64 rows of 201,088 with histories of 50-4,096, 50 biases and a mask, fp32: 47 us, 2.2 TB/s (the
+// bytes alone take 16); one row with a history of 500: 9 us one call after another. Segments of 4,096 to 16,384
+// entries on 128 to 1,024 threads, with one to four words of history under way before the table is cleared, all took
+// 45 to 57 us for the 64 rows.
 #pragma once
 
 #include <limits.h>
@@ -15,7 +21,8 @@
 namespace cb200 {
 
 // Entries of a segment: 4 or 16 a thread. Few rows are cut finer, so that they reach all SMs; many rows coarser, since
-// every segment reads its row's history (a row of 201,088: 24.6 us with 4,096 entries, XXX with 1,024).
+// every segment reads its row's history (rows of 201,088 with 1,024 and with 4,096 entries: one 12 and 16 us, two 14 and 18,
+// four 16 and 18, twelve 25 and 20, sixty-four 78 and 47, by events around a graph).
 constexpr int kLogitsThreads = 256, kLogitsShort = 4 * kLogitsThreads, kLogitsLong = 16 * kLogitsThreads;
 // A token's word in the table of its segment: it occurs in the prompt, it has a bias, and how often it occurs after that.
 constexpr unsigned kHeardBit = 0x80000000u, kBiasBit = 0x40000000u, kTimes = 0x3fffffffu;

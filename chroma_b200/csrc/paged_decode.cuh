@@ -10,6 +10,9 @@
 // in registers, and the warps' results are merged in shared memory at the end of an item. An item that lies within one
 // CTA is finished there; the others leave fp32 partial results, and the CTAs of an item's parts follow from the cut, so
 // k_paged_join needs no flags or counters.
+//
+// Bound by HBM for long caches: keys and values are read once, and 8 query heads share them (8 multiply-adds a byte, far below what the tensor core
+// could do). Short ones are bound by the latency of lengths, table, keys, values, join, each read after the other.
 #pragma once
 
 #include "mma.cuh"
@@ -478,10 +481,10 @@ k_paged_decode(PagedDecodeArgs p) {
 // multiple of 16 rows: U positions of K and of V per stage, 128-byte swizzle, read with ldmatrix (transposed for V).
 // Every warp has its own ring and issues its own loads, kStages ahead, so there is no barrier between warps, and two to
 // three times as many bytes are under way as registers could hold: bound by HBM. 128 sequences of 1,024-4,096 positions
-// (64/8 heads of 64): 115 us of kernel, 121 with its launches and the join, 5.6 TB/s (k_paged_decode 142); a ring of
-// cp.async took 194. Eight warps on an SM are enough: sixteen with half the positions a stage took as long.
+// (64/8 heads of 64): 115 us of kernel, 120 with its launches and the join, 5.6 TB/s (k_paged_decode 142); two of 40,001 and
+// 131,071 (32/8 heads of 128): 139 us, 6.05 TB/s. A ring of cp.async took 194 for the first. Eight warps on an SM are enough: sixteen with half the positions a stage took as long.
 template <int DC> struct DecodeRing {
-        static constexpr int U = DC == 2 ? 32 : 16, kWarps = 4, kStages = 3, kTile = U * 64 * DC, kStage = 2 * kTile;
+    static constexpr int U = DC == 2 ? 32 : 16, kWarps = 4, kStages = 3, kTile = U * 64 * DC, kStage = 2 * kTile;
     static constexpr int kSmem = 1024 + kWarps * (kStages * kStage + 8 * kMergeDims * 4);
 };
 

@@ -5,12 +5,15 @@
 // 8 of them, of several consecutive tokens. Units of 32 positions are dealt to the 8 warps of a CTA, and each warp works on
 // its own. The unit's keys are copied to shared memory, 64 values of a row at a time, row by row; then a lane has one key: it
 // walks the key's row there and multiplies each 16-byte word with the same words of the 8 query rows, which all lanes read
-// from the same place, so a score needs no exchange between lanes. (Rows of 64 bytes are read by their lanes directly.) Values are read with a row spread over `kWords` lanes, the
-// 8 weights of a key in two words of shared memory. Single tokens are cut, merged and joined as in paged_decode.cuh.
+// from the same place, so a score needs no exchange between lanes. (Rows of 64 bytes are read by their lanes directly.)
+// Values are read with a row spread over `kWords` lanes, the 8 weights of a key in two words of shared memory. Single tokens
+// are cut, merged and joined as in paged_decode.cuh.
 //
 // What bounds it: where caches are short, the latency of five dependent reads; else shared memory and its load instructions
 // (of 32 keys and 64 values: 1,024 FMA instructions a warp, and about 400 cycles of the SM's load pipe; with each lane reading
-// its own key from global memory, and weights passed by shuffles, it was 870).
+// its own key from global memory, and weights passed by shuffles, it was 870). 64 sequences of 500-2,000 positions with 64/8
+// heads of 64: 109 us, 12 TFLOP/s (143 in that form); two of 30,000-60,000 with 8/2 heads of 128: 78 us; two prompts of 1,000
+// with 16/4 heads of 64: 297 us. One sequence of 160 with 8 heads of 16: 7.7 us one call after another.
 #pragma once
 
 #include <limits.h>

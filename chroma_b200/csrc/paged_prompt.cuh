@@ -22,9 +22,11 @@
 // What bounds it: the exponentials and what goes with them on 128 rows of one thread each, in turn with the products
 // (clock stamps per tile of 64-value heads: 1,400 cycles of exponentials, 650 around them, 1,000 waiting; the
 // special-function unit is busy half of the time, the tensor core a quarter). Four prompts of 2,048 tokens, 64/8 heads of
-// 64: 300 us, 458 TFLOP/s; 8,192 tokens after 8,001 in a window of 4,096, 32/8 heads of 128: 586 us, 939 TFLOP/s. Tried
-// and slower: a quarter to a half of the exponentials as a polynomial on the FMA pipe (305 to 354 us; issue slots), the
-// issuing warp taking whatever is ready first (301 and 653 us), the two tiles' exponentials in turn (313 and 604 us).
+// 64: 276 us, 498 TFLOP/s (266 one call after another); 8,192 tokens after 8,001 in a window of 4,096, 32/8 heads of 128:
+// 580 us, 949 TFLOP/s, and 633 once the GPU is at its power limit; two prompts of 4,096 with 32/8 heads of 128: 297 us.
+// Tried when those two took 300 and 586 us, and slower: a quarter to a half of the exponentials as a polynomial on the FMA
+// pipe (305 to 354 us; issue slots), the issuing warp taking whatever is ready first (301 and 653 us), a second issuing
+// warp (317 and 640 us), the two tiles' exponentials in turn (313 and 604 us).
 //
 // A position that no row may see costs nothing (whole tiles are passed over) or a mask of 128 bits per row, applied only
 // to the tiles that need it. Values behind the end of a sequence are cleared in shared memory, since what lies there may
@@ -32,7 +34,7 @@
 // protection against infinities: a row whose result is not finite is computed again, key by key.
 //
 // Where there are few items (a short chunk after a long cache), the keys of each are split over several CTAs, which leave
-// fp32 partial results for k_prompt_join.
+// fp32 partial results for k_prompt_join (16 tokens after 16,000, 64/8 heads of 64: 69 us, without splits 203).
 //
 // All waits are bounded (tma.cuh).
 #pragma once
@@ -575,7 +577,7 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
                 const float neg = m_new == -INFINITY ? 0.f : -m_new;
                 m_run = m_new;
                 // P's own columns, and O, are this warpgroup's once the product before is done; without own columns, S said so.
-                // Waited for here and not before P is stored, it also keeps the two warpgroups half a period apart (300 us
+                // Waited for here and not before P is stored, it also keeps the two warpgroups half a period apart (then 300 us
                 // for the four prompts of 2,048 tokens, against 334).
                 if (kOwnP) {
                     if (uses > 1 && !mbar_wait(&o_done[k], unsigned(uses & 1), p.error)) abort_flag = 1;
