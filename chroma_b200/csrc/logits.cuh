@@ -16,7 +16,7 @@
 
 #include <limits.h>
 
-#include "common.cuh"
+#include "paged.cuh"
 
 namespace cb200 {
 
@@ -38,6 +38,9 @@ struct LogitsArgs {
     const unsigned* mask;
     unsigned long long* best;  // [rows][segments] argmax keys, or nullptr
     int64_t stride, out_stride, history_stride, bias_ids_stride, bias_stride, mask_stride;
+    unsigned* special;         // [rows][special_stride] bits: entries that occurred or have a bias; or nullptr
+    int special_stride, best_at;  // best_at: this launch's first segment of `best`
+    FastDiv by_ctas;              // d: CTAs that share a row's words of 32 entries, in turn
     int vocab, width, biases, segments;
     int vector, history_vector;  // rows of logits and out, of the history, are 16-byte aligned
 };
@@ -56,12 +59,12 @@ __device__ __noinline__ float divided_anyhow(float a, float b) { return __fdiv_r
 
 // The sum of the biases of token `begin` + i, in the order of the row's list. `listed` of the list lie in the segment that
 // begins there; as many as there is room for are in shared memory, in any order, with their places in the list.
-__device__ __noinline__ float bias_sum(const int* all_ids, const float* all, int biases, int begin, int i, int listed, const int* ids,
+__device__ __noinline__ float bias_sum(const int* all_ids, const float* all, int biases, int token, int i, int listed, const int* ids,
                                        const int* places, const float* values) {
     float sum = 0.f;
     if (listed > kLogitsListed) {
         for (int j = 0; j < biases; ++j)
-            if (all_ids[j] - begin == i) sum = __fadd_rn(sum, all[j]);
+            if (all_ids[j] == token) sum = __fadd_rn(sum, all[j]);
         return sum;
     }
     for (int last = -1;;) {
@@ -74,8 +77,8 @@ __device__ __noinline__ float bias_sum(const int* all_ids, const float* all, int
     }
 }
 
-template <typename T, int kSegment> __global__ void __launch_bounds__(kLogitsThreads, 5) k_logits(LogitsArgs a) {
-    constexpr int kPer = 16 / sizeof(T);
+template <typename T> __global__ void __launch_bounds__(kLogitsThreads, 5) k_logits(LogitsArgs a) {
+    constexpr int kPer = 16 / sizeof(T), kSegment = kLogitsShort;
     __shared__ __align__(16) unsigned counts[kSegment];
     __shared__ unsigned special[kSegment / 32];  // entries that occurred or have a bias: they are left to the second pass
     __shared__ uint16_t specials[kSegment];
@@ -232,7 +235,7 @@ template <typename T, int kSegment> __global__ void __launch_bounds__(kLogitsThr
                 x = x > 0.f ? divided_anyhow(x, r) : __fmul_rn(x, r);
                 if (times) x = __fsub_rn(__fsub_rn(x, __fmul_rn(f, float(times))), pr);
             }
-            if (c & kBiasBit) x = __fadd_rn(x, bias_sum(a.bias_ids + row * a.bias_ids_stride, a.bias + row * a.bias_stride, a.biases, begin, i, s_listed, listed_ids, listed_at, listed));
+            if (c & kBiasBit) x = __fadd_rn(x, bias_sum(a.bias_ids + row * a.bias_ids_stride, a.bias + row * a.bias_stride, a.biases, begin + i, i, s_listed, listed_ids, listed_at, listed));
             x = finished(x, allowed_at(i));
             Store<T>::store(out + i, x);
             // Not in ascending order: of equals the lower index.
@@ -254,6 +257,229 @@ template <typename T, int kSegment> __global__ void __launch_bounds__(kLogitsThr
         for (int w = 1; w < kLogitsThreads / 32; ++w) best = keys[w] > best ? keys[w] : best;
         a.best[int64_t(row) * a.segments + blockIdx.x] = best;
     }
+}
+
+// Entries of many rows that occurred or have a bias. A row's words of 32 entries are dealt out to `by_ctas.d` CTAs, so that the
+// low ids, which occur most, meet all of them. Each CTA counts its share of the history in a hash table that has room for every
+// entry that can come (at least a quarter stays empty), finishes those entries, and leaves bits of where they are.
+constexpr int kHeardThreads = 512, kHeardSlots = 8192, kHeardMost = 6144, kHeardWords = 8192;
+struct HeardTable {
+    int ids[kHeardSlots];
+    unsigned counts[kHeardSlots];
+    uint16_t used[kHeardMost];
+    int listed_ids[kLogitsListed], listed_at[kLogitsListed];
+    float listed[kLogitsListed];
+    unsigned long long keys[kHeardThreads / 32];
+    int n_listed, n_used;
+    unsigned special[];  // words of the CTA
+};
+
+template <typename T> __global__ void __launch_bounds__(kHeardThreads, 2) k_logits_heard(LogitsArgs a) {
+    extern __shared__ __align__(16) uint8_t heard_smem[];
+    HeardTable& sm = *reinterpret_cast<HeardTable*>(heard_smem);
+    asm volatile("griddepcontrol.launch_dependents;" :::);
+    const int row = blockIdx.y, ctas = a.by_ctas.d, words = (a.special_stride + ctas - 1) / ctas;
+    const T* in = static_cast<const T*>(a.logits) + row * a.stride;
+    T* out = static_cast<T*>(a.out) + row * a.out_stride;
+    const int* history = a.history + row * a.history_stride;
+    const int* bias_ids = a.bias_ids + row * a.bias_ids_stride;
+    const float* bias = a.bias + row * a.bias_stride;
+    const auto tokens = [&](int i) {  // entries i .. i + 3
+        if (a.history_vector && i + 4 <= a.width) return __ldg(reinterpret_cast<const int4*>(history + i));
+        return make_int4(i < a.width ? __ldg(history + i) : -1, i + 1 < a.width ? __ldg(history + i + 1) : -1,
+                         i + 2 < a.width ? __ldg(history + i + 2) : -1, i + 3 < a.width ? __ldg(history + i + 3) : -1);
+    };
+    int4 next = make_int4(-1, -1, -1, -1);
+    if (a.history) next = tokens(4 * threadIdx.x);
+    const int len = a.history ? min(max(a.lengths[row], 0), a.width) : 0, prompt = a.history && a.prompts ? a.prompts[row] : 0;
+    for (int i = 4 * threadIdx.x; i < kHeardSlots; i += 4 * kHeardThreads) {
+        *reinterpret_cast<int4*>(sm.ids + i) = make_int4(-1, -1, -1, -1);
+        *reinterpret_cast<uint4*>(sm.counts + i) = make_uint4(0, 0, 0, 0);
+    }
+    for (int i = threadIdx.x; i < words; i += kHeardThreads) sm.special[i] = 0;
+    if (threadIdx.x == 0) sm.n_listed = sm.n_used = 0;
+    __syncthreads();
+    // The slot of an entry of this CTA, -1 for others.
+    const auto slot = [&](int token) {
+        if (unsigned(token) >= unsigned(a.vocab)) return -1;
+        const unsigned word = unsigned(token) >> 5, at = a.by_ctas.div(word);
+        if (word - at * ctas != blockIdx.x) return -1;
+        unsigned h = unsigned(token) * 2654435761u >> 19;  // 13 bits of the golden ratio's multiple
+        while (true) {
+            int id = *reinterpret_cast<volatile int*>(sm.ids + h);
+            if (id == -1) {
+                id = atomicCAS(sm.ids + h, -1, token);
+                if (id == -1) {
+                    sm.used[atomicAdd(&sm.n_used, 1)] = uint16_t(h);
+                    atomicOr(&sm.special[at], 1u << (token & 31));
+                    return int(h);
+                }
+            }
+            if (id == token) return int(h);
+            h = (h + 1) % kHeardSlots;
+        }
+    };
+    const auto hear = [&](int i, int token) {
+        const int h = i < len ? slot(token) : -1;
+        if (h >= 0) {
+            if (i < prompt) atomicOr(&sm.counts[h], kHeardBit);
+            else atomicAdd(&sm.counts[h], 1u);
+        }
+    };
+    for (int i = 4 * threadIdx.x; i < len; i += 4 * kHeardThreads) {
+        const int4 x = next;
+        if (i + 4 * kHeardThreads < len) next = tokens(i + 4 * kHeardThreads);
+        hear(i, x.x);
+        hear(i + 1, x.y);
+        hear(i + 2, x.z);
+        hear(i + 3, x.w);
+    }
+    if (a.bias_ids)
+        for (int i = threadIdx.x; i < a.biases; i += kHeardThreads) {
+            const int h = slot(__ldg(bias_ids + i));
+            if (h < 0) continue;
+            atomicOr(&sm.counts[h], kBiasBit);
+            const int at = atomicAdd(&sm.n_listed, 1);
+            if (at < kLogitsListed) {
+                sm.listed_ids[at] = h;
+                sm.listed_at[at] = i;
+                sm.listed[at] = bias[i];
+            }
+        }
+    __syncthreads();
+    for (int i = threadIdx.x, word; i < words && (word = i * ctas + blockIdx.x) < a.special_stride; i += kHeardThreads)
+        a.special[int64_t(row) * a.special_stride + word] = sm.special[i];
+    const float temp = a.temperature ? a.temperature[row] : 0.f, r = a.repetition ? a.repetition[row] : 1.f;
+    const float f = a.frequency ? a.frequency[row] : 0.f, pr = a.presence ? a.presence[row] : 0.f;
+    unsigned long long best = 0;
+    for (int k = threadIdx.x; k < sm.n_used; k += kHeardThreads) {
+        const int h = sm.used[k], i = sm.ids[h];
+        const unsigned c = sm.counts[h], times = c & kTimes;
+        const unsigned on = a.mask ? __ldg(a.mask + row * a.mask_stride + (i >> 5)) >> (i & 31) & 1 : 1u;
+        float x = Store<T>::load(in + i);
+        if (c & ~kBiasBit) {
+            x = x > 0.f ? divided_anyhow(x, r) : __fmul_rn(x, r);
+            if (times) x = __fsub_rn(__fsub_rn(x, __fmul_rn(f, float(times))), pr);
+        }
+        if (c & kBiasBit) x = __fadd_rn(x, bias_sum(bias_ids, bias, a.biases, i, h, sm.n_listed, sm.listed_ids, sm.listed_at, sm.listed));
+        if (temp != 0.f) x = divided_anyhow(x, temp);
+        x = on ? Store<T>::round(x) : -INFINITY;
+        Store<T>::store(out + i, x);
+        const unsigned long long key = argmax_key(x + 0.0f, i);  // + 0: a negative zero equals a positive one
+        best = key > best ? key : best;
+    }
+    if (!a.best) return;
+    for (int o = 16; o; o >>= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
+        best = other > best ? other : best;
+    }
+    if ((threadIdx.x & 31) == 0) sm.keys[threadIdx.x >> 5] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kHeardThreads / 32; ++w) best = sm.keys[w] > best ? sm.keys[w] : best;
+        a.best[int64_t(row) * a.segments + a.best_at + blockIdx.x] = best;
+    }
+}
+
+// The largest of three, or NaN if one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
+
+// The entries of many rows that neither occurred nor have a bias, while the launch before still finds out which did (what
+// is read of the others before its end is not used). 16 entries a thread stay in registers until the segment's largest
+// is known; only then the few threads that hold it look where.
+template <typename T> __global__ void __launch_bounds__(kLogitsThreads, 4) k_logits_rest(LogitsArgs a) {
+    constexpr int kPer = 16 / sizeof(T), kWords = kLogitsLong / (kPer * kLogitsThreads);
+    __shared__ __align__(16) unsigned tops[kLogitsThreads / 32];
+    __shared__ int s_where;
+    asm volatile("griddepcontrol.launch_dependents;" :::);
+    const int row = blockIdx.y, begin = blockIdx.x * kLogitsLong, n = min(kLogitsLong, a.vocab - begin);
+    const T* in = static_cast<const T*>(a.logits) + row * a.stride + begin;
+    T* out = static_cast<T*>(a.out) + row * a.out_stride + begin;
+    const float temp = a.temperature ? a.temperature[row] : 0.f;
+    const bool usual_temp = fabsf(temp) > 0x1p-30f && fabsf(temp) < 0x1p30f;
+    const float per_temp = __frcp_rn(temp);
+    alignas(16) T raw[kWords][kPer];
+    unsigned on[kWords], left[kWords];
+#pragma unroll
+    for (int v = 0; v < kWords; ++v) {
+        const int i = kPer * (threadIdx.x + v * kLogitsThreads);
+        if (a.vector && i + kPer <= n) *reinterpret_cast<uint4*>(raw[v]) = *reinterpret_cast<const uint4*>(in + i);
+        else
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) raw[v][e] = i + e < n ? in[i + e] : T(0.f);
+        on[v] = a.mask && i < n ? __ldg(a.mask + row * a.mask_stride + ((begin + i) >> 5)) : ~0u;
+        left[v] = 0;
+    }
+    if (a.special) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+#pragma unroll
+        for (int v = 0; v < kWords; ++v) {
+            const int i = kPer * (threadIdx.x + v * kLogitsThreads);
+            if (i < n) left[v] = __ldcg(a.special + int64_t(row) * a.special_stride + ((begin + i) >> 5));
+        }
+    }
+    if (threadIdx.x == 0) s_where = INT_MAX;
+    float x[kWords][kPer], top = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < kWords; ++v) {
+        const int i = kPer * (threadIdx.x + v * kLogitsThreads);
+        const unsigned shift = i & 31, all = (1u << kPer) - 1;
+        unsigned skip = left[v] >> shift & all;
+        if (i + kPer > n) skip |= i < n ? all << (n - i) & all : all;
+        const unsigned open = on[v] >> shift & ~skip;
+        float low = INFINITY, high = 0.f;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            x[v][e] = Store<T>::load(raw[v] + e);
+            low = fminf(low, fabsf(x[v][e]));
+            high = fmaxf(high, fabsf(x[v][e]));
+        }
+        if (temp != 0.f) {
+            if (usual_temp && low > 0x1p-60f && high < 0x1p60f)
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) x[v][e] = divided(x[v][e], temp, per_temp);
+            else
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) x[v][e] = divided_anyhow(x[v][e], temp);
+        }
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            x[v][e] = open & (1u << e) ? Store<T>::round(x[v][e]) : -INFINITY;
+            Store<T>::store(raw[v] + e, x[v][e]);
+        }
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2) top = max3_nan(top, x[v][e], x[v][e + 1]);
+        if (!skip && a.vector) *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(raw[v]);
+        else
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                if (!(skip & (1u << e))) out[i + e] = raw[v][e];
+    }
+    if (!a.best) return;
+    const unsigned key = unsigned(argmax_key(top + 0.0f, 0) >> 32);  // + 0: a negative zero equals a positive one
+    const unsigned warp_key = __reduce_max_sync(0xffffffffu, key);
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = warp_key;
+    __syncthreads();
+    unsigned best = 0;
+#pragma unroll
+    for (int w = 0; w < kLogitsThreads / 32; ++w) best = max(best, tops[w]);
+    if (key == best) {
+        int where = INT_MAX;
+#pragma unroll
+        for (int v = kWords - 1; v >= 0; --v)
+#pragma unroll
+            for (int e = kPer - 1; e >= 0; --e)
+                if (x[v][e] == top || (x[v][e] != x[v][e] && top != top)) where = kPer * (threadIdx.x + v * kLogitsThreads) + e;
+        atomicMin(&s_where, where);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0)
+        a.best[int64_t(row) * a.segments + blockIdx.x] =
+            (static_cast<unsigned long long>(best) << 32) | (0xffffffffu - static_cast<unsigned>(begin + s_where));
 }
 
 // The best of a row's segments; one warp per row.

@@ -4,6 +4,7 @@
 
 #include <cuda.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdio>
 #include <stdexcept>
@@ -369,6 +370,19 @@ template <typename K> size_t shared_marks(K kernel, const chroma_b200_pages& p) 
     return bytes;
 }
 
+// Bytes of the best of every segment of every row: of k_logits, or of k_logits_rest and k_logits_heard.
+int64_t logits_best_bytes(int64_t rows, int64_t vocab) { return rows * ((vocab + kLogitsShort - 1) / kLogitsShort + 1) * 8; }
+
+// CTAs that share a row in k_logits_heard: two a SM at once, and as many as it takes for every entry that can come to have a
+// slot, and every word of bits a place; no more than there are long segments.
+int heard_ctas(const chroma_b200_logits& g) {
+    const int64_t words = (int64_t(g.vocab) + 31) / 32, come = (g.history ? int64_t(g.width) : 0) + (g.bias_ids ? g.biases : 0);
+    int64_t ctas = 2 * sm_count() / g.rows, need = (words + kHeardWords - 1) / kHeardWords;
+    if (come > kHeardMost) need = std::max(need, (words * 32 + kHeardMost - 1) / kHeardMost);
+    ctas = std::max(ctas, need);
+    return int(std::max<int64_t>(1, std::min(ctas, std::max(need, (words + 127) / 128))));
+}
+
 dim3 table_grid(const chroma_b200_pages& p) { return dim3(unsigned((p.width + 255) / 256), unsigned(p.slots)); }
 
 }  // namespace
@@ -516,7 +530,7 @@ int chroma_b200_compact_pages(const chroma_b200_pages* p, int32_t* new_table, in
 }
 
 int64_t chroma_b200_logits_workspace(int32_t rows, int32_t vocab) {
-    return rows < 0 || vocab < 0 ? -1 : int64_t(rows) * ((int64_t(vocab) + kLogitsShort - 1) / kLogitsShort) * 8;
+    return rows < 0 || vocab < 0 ? -1 : logits_best_bytes(rows, vocab) + int64_t(rows) * ((int64_t(vocab) + 31) / 32) * 4;
 }
 
 int chroma_b200_process_logits(const chroma_b200_logits* g, void* stream, char* err, size_t err_len) {
@@ -528,7 +542,7 @@ int chroma_b200_process_logits(const chroma_b200_logits* g, void* stream, char* 
         want(g->rows <= 65535, "at most 65,535 rows");
         if (!g->rows) return;
         want(g->logits && g->out, "null argument");
-        want(!g->argmax || (g->workspace && g->workspace_bytes >= chroma_b200_logits_workspace(g->rows, g->vocab)),
+        want(!(g->argmax || g->history || g->bias_ids) || (g->workspace && g->workspace_bytes >= chroma_b200_logits_workspace(g->rows, g->vocab)),
              "workspace too small");
         const auto s = cudaStream_t(stream);
         LogitsArgs a{};
@@ -544,11 +558,27 @@ int chroma_b200_process_logits(const chroma_b200_logits* g, void* stream, char* 
         a.history_vector = aligned16(g->history) && (g->rows == 1 || g->history_stride % 4 == 0);
         // Long segments once they alone give every SM two CTAs (both measured beside kLogitsShort).
         const bool few = int64_t(g->rows) * ((g->vocab + kLogitsLong - 1) / kLogitsLong) < 2 * sm_count();
-        const int segment = few ? kLogitsShort : kLogitsLong;
-        a.segments = (g->vocab + segment - 1) / segment;
+        const int short_segments = (g->vocab + kLogitsShort - 1) / kLogitsShort, long_segments = (g->vocab + kLogitsLong - 1) / kLogitsLong;
         by_type(g->storage, [&](auto t) {
-            const auto kernel = few ? k_logits<decltype(t), kLogitsShort> : k_logits<decltype(t), kLogitsLong>;
-            launch(s, dim3(unsigned(a.segments), unsigned(g->rows)), dim3(kLogitsThreads), 0, kernel, a);
+            using T = decltype(t);
+            const dim3 threads(kLogitsThreads), rest(unsigned(long_segments), unsigned(g->rows));
+            if (few) {
+                a.segments = short_segments;
+                launch(s, dim3(unsigned(short_segments), unsigned(g->rows)), threads, 0, k_logits<T>, a);
+                return;
+            }
+            a.segments = long_segments;
+            if (!a.history && !a.bias_ids) return launch(s, rest, threads, 0, k_logits_rest<T>, a);
+            a.special_stride = (g->vocab + 31) / 32;
+            a.special = reinterpret_cast<unsigned*>(static_cast<char*>(g->workspace) + logits_best_bytes(g->rows, g->vocab));
+            const int ctas = heard_ctas(*g);
+            a.by_ctas = FastDiv(uint32_t(ctas));
+            a.best_at = long_segments;
+            a.segments += ctas;
+            const int smem = int(sizeof(HeardTable)) + (a.special_stride + ctas - 1) / ctas * 4;
+            check(cudaFuncSetAttribute(k_logits_heard<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "smem attribute");
+            launch(s, dim3(unsigned(ctas), unsigned(g->rows)), dim3(kHeardThreads), smem, k_logits_heard<T>, a);
+            launch_after(s, rest, threads, k_logits_rest<T>, a);
         });
         if (g->argmax) launch_after(s, dim3(unsigned(g->rows)), dim3(32), k_logits_pick, a.best, a.segments, g->argmax);
     });

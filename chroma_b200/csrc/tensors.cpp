@@ -295,6 +295,8 @@ PyObject* process_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (argmax) {
         best = call.empty({rows}, at::kLong);
         g.argmax = best.data_ptr<int64_t>();
+    }
+    if (argmax || g.history || g.bias_ids) {
         g.workspace_bytes = native.logits_workspace(g.rows, g.vocab);
         room = call.empty({g.workspace_bytes}, at::kByte);
         g.workspace = room.data_ptr();

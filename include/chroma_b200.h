@@ -314,7 +314,7 @@ typedef struct chroma_b200_logits {
     const int32_t *bias_ids;      /* [rows][biases], or NULL */
     const float *bias;            /* [rows][biases] */
     const int32_t *mask;          /* [rows][(vocab + 31) / 32] bits, 1 = allowed, rows `mask_stride` apart, or NULL */
-    void *workspace;              /* with argmax: chroma_b200_logits_workspace bytes */
+    void *workspace;              /* with argmax, history or bias_ids: chroma_b200_logits_workspace bytes */
     int64_t stride, out_stride, history_stride, bias_ids_stride, bias_stride, mask_stride, workspace_bytes;
     int32_t storage, rows, vocab, width, biases;
 } chroma_b200_logits;
