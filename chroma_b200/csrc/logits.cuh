@@ -1,28 +1,32 @@
 // What is done to logits before a token is chosen from them: penalties for tokens that occurred, biases, temperature,
 // the mask of a grammar, and the greedy choice.
 //
-// One CTA takes a segment of one row: it counts the row's history into a table of its segment in shared memory, adds the
-// biases of its segment in list order, and passes over the logits once, 16 bytes a thread at a time. No table of counts is
-// kept between calls. The arithmetic is rounded operation by operation (no fused multiply-add), so that results do not
-// depend on how the compiler groups it, and equal logits stay equal. The best of each segment is left for a second, small
-// launch.
+// Few rows (k_logits): one CTA takes a segment of one row, counts the row's history into a table of its segment in shared
+// memory, adds the biases of its segment in list order, and passes over the logits once, 16 bytes a thread. Many rows: reading
+// the history once for every segment would cost more than the logits, so k_logits_heard finishes the entries that
+// occurred or have a bias, through a hash table, and leaves their bits; k_logits_rest streams the others. The best of each
+// segment is left for a last, small launch. No table of counts is kept between calls. The arithmetic is rounded operation by
+// operation (no fused multiply-add), so that results do not depend on how the compiler groups it, and equal logits stay equal.
 //
-// Bound by latency: each CTA's chain of row length, history, table, logits, best of the segment is longer than its
-// share of the stream. 64 rows of 201,088 with histories of 50-4,096, 50 biases and a mask, fp32: 47 us, 2.2 TB/s (the
-// bytes alone take 16); one row with a history of 500: 9 us one call after another. Segments of 4,096 to 16,384
-// entries on 128 to 1,024 threads, with one to four words of history under way before the table is cleared, all took
-// 45 to 57 us for the 64 rows.
+// Bound: one row by the latency of a few dependent reads (history of 500: 9 us one call after another, as long as the
+// host's call). 64 rows of 201,088 with histories of 50-4,096, 50 biases and a mask, fp32: 32 us, 3.2 TB/s, where the bytes
+// alone take 16: 8 us are the chain of row length, history, table, logits of the first launch, under which only the first
+// segments of the second are read, and the second one issues 20 instructions an entry (five of them the division by the temperature);
+// 128 rows 55 us. All in one launch, with segments of 4,096 to 16,384 entries on 128 to 1,024 threads, took 45 to 57 us for
+// the 64 rows; a table with a place for each of 16,384 entries in place of the hash table 47.
 #pragma once
 
 #include <limits.h>
+
+#include <type_traits>
 
 #include "paged.cuh"
 
 namespace cb200 {
 
-// Entries of a segment: 4 or 16 a thread. Few rows are cut finer, so that they reach all SMs; many rows coarser, since
-// every segment reads its row's history (rows of 201,088 with 1,024 and with 4,096 entries: one 12 and 16 us, two 14 and 18,
-// four 16 and 18, twelve 25 and 20, sixty-four 78 and 47, by events around a graph).
+// Entries of a segment: 4 or 16 a thread. Few rows are cut finer, so that they reach all SMs. (Rows of 201,088, all in one
+// launch with 1,024 entries a segment and in two with 4,096: one 12 and 14 us, two 14 and 16, four 16 and 16, six 18 and 18,
+// twelve 25 and 18, sixty-four 80 and 33, by events around a graph.)
 constexpr int kLogitsThreads = 256, kLogitsShort = 4 * kLogitsThreads, kLogitsLong = 16 * kLogitsThreads;
 // A token's word in the table of its segment: it occurs in the prompt, it has a bias, and how often it occurs after that.
 constexpr unsigned kHeardBit = 0x80000000u, kBiasBit = 0x40000000u, kTimes = 0x3fffffffu;
@@ -262,7 +266,7 @@ template <typename T> __global__ void __launch_bounds__(kLogitsThreads, 5) k_log
 // Entries of many rows that occurred or have a bias. A row's words of 32 entries are dealt out to `by_ctas.d` CTAs, so that the
 // low ids, which occur most, meet all of them. Each CTA counts its share of the history in a hash table that has room for every
 // entry that can come (at least a quarter stays empty), finishes those entries, and leaves bits of where they are.
-constexpr int kHeardThreads = 512, kHeardSlots = 8192, kHeardMost = 6144, kHeardWords = 8192;
+constexpr int kHeardThreads = 1024, kHeardSlots = 8192, kHeardMost = 6144, kHeardWords = 8192;
 struct HeardTable {
     int ids[kHeardSlots];
     unsigned counts[kHeardSlots];
@@ -274,7 +278,7 @@ struct HeardTable {
     unsigned special[];  // words of the CTA
 };
 
-template <typename T> __global__ void __launch_bounds__(kHeardThreads, 2) k_logits_heard(LogitsArgs a) {
+template <typename T> __global__ void __launch_bounds__(kHeardThreads, 1) k_logits_heard(LogitsArgs a) {
     extern __shared__ __align__(16) uint8_t heard_smem[];
     HeardTable& sm = *reinterpret_cast<HeardTable*>(heard_smem);
     asm volatile("griddepcontrol.launch_dependents;" :::);
@@ -391,7 +395,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 // The entries of many rows that neither occurred nor have a bias, while the launch before still finds out which did (what
 // is read of the others before its end is not used). 16 entries a thread stay in registers until the segment's largest
 // is known; only then the few threads that hold it look where.
-template <typename T> __global__ void __launch_bounds__(kLogitsThreads, 4) k_logits_rest(LogitsArgs a) {
+template <typename T> __global__ void __launch_bounds__(kLogitsThreads, 5) k_logits_rest(LogitsArgs a) {
     constexpr int kPer = 16 / sizeof(T), kWords = kLogitsLong / (kPer * kLogitsThreads);
     __shared__ __align__(16) unsigned tops[kLogitsThreads / 32];
     __shared__ int s_where;
@@ -402,63 +406,79 @@ template <typename T> __global__ void __launch_bounds__(kLogitsThreads, 4) k_log
     const float temp = a.temperature ? a.temperature[row] : 0.f;
     const bool usual_temp = fabsf(temp) > 0x1p-30f && fabsf(temp) < 0x1p30f;
     const float per_temp = __frcp_rn(temp);
-    alignas(16) T raw[kWords][kPer];
-    unsigned on[kWords], left[kWords];
-#pragma unroll
-    for (int v = 0; v < kWords; ++v) {
-        const int i = kPer * (threadIdx.x + v * kLogitsThreads);
-        if (a.vector && i + kPer <= n) *reinterpret_cast<uint4*>(raw[v]) = *reinterpret_cast<const uint4*>(in + i);
-        else
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) raw[v][e] = i + e < n ? in[i + e] : T(0.f);
-        on[v] = a.mask && i < n ? __ldg(a.mask + row * a.mask_stride + ((begin + i) >> 5)) : ~0u;
-        left[v] = 0;
-    }
-    if (a.special) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr unsigned kAll = (1u << kPer) - 1;
+    const int at = kPer * threadIdx.x, shift = at & 31;  // the same bits of a word in every vector
+    float x[kWords][kPer], top = -INFINITY;
+    const auto pass = [&](auto whole) {  // whole: every vector of 16 bytes lies in the row, and is aligned
+        constexpr bool kWhole = decltype(whole)::value;
+        alignas(16) T raw[kWords][kPer];
+        unsigned on[kWords], left[kWords];
+        const T* from = in + at;
+        const unsigned* mask = a.mask + row * a.mask_stride + ((begin + at) >> 5);
 #pragma unroll
         for (int v = 0; v < kWords; ++v) {
-            const int i = kPer * (threadIdx.x + v * kLogitsThreads);
-            if (i < n) left[v] = __ldcg(a.special + int64_t(row) * a.special_stride + ((begin + i) >> 5));
-        }
-    }
-    if (threadIdx.x == 0) s_where = INT_MAX;
-    float x[kWords][kPer], top = -INFINITY;
+            constexpr int kStep = kPer * kLogitsThreads;
+            if (kWhole) *reinterpret_cast<uint4*>(raw[v]) = *reinterpret_cast<const uint4*>(from + v * kStep);
+            else
 #pragma unroll
-    for (int v = 0; v < kWords; ++v) {
-        const int i = kPer * (threadIdx.x + v * kLogitsThreads);
-        const unsigned shift = i & 31, all = (1u << kPer) - 1;
-        unsigned skip = left[v] >> shift & all;
-        if (i + kPer > n) skip |= i < n ? all << (n - i) & all : all;
-        const unsigned open = on[v] >> shift & ~skip;
+                for (int e = 0; e < kPer; ++e) raw[v][e] = at + v * kStep + e < n ? from[v * kStep + e] : T(0.f);
+            on[v] = a.mask && (kWhole || at + v * kStep < n) ? __ldg(mask + v * (kStep / 32)) : ~0u;
+            left[v] = 0;
+        }
+        if (a.special) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            const unsigned* special = a.special + int64_t(row) * a.special_stride + ((begin + at) >> 5);
+#pragma unroll
+            for (int v = 0; v < kWords; ++v)
+                if (kWhole || at + v * kPer * kLogitsThreads < n) left[v] = __ldcg(special + v * (kPer * kLogitsThreads / 32));
+        }
         float low = INFINITY, high = 0.f;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            x[v][e] = Store<T>::load(raw[v] + e);
-            low = fminf(low, fabsf(x[v][e]));
-            high = fmaxf(high, fabsf(x[v][e]));
-        }
+        for (int v = 0; v < kWords; ++v)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                x[v][e] = Store<T>::load(raw[v] + e);
+                if (kWhole || at + v * kPer * kLogitsThreads + e < n) {
+                    low = fminf(low, fabsf(x[v][e]));
+                    high = fmaxf(high, fabsf(x[v][e]));
+                }
+            }
         if (temp != 0.f) {
             if (usual_temp && low > 0x1p-60f && high < 0x1p60f)
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) x[v][e] = divided(x[v][e], temp, per_temp);
+                for (int v = 0; v < kWords; ++v)
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) x[v][e] = divided(x[v][e], temp, per_temp);
             else
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) x[v][e] = divided_anyhow(x[v][e], temp);
+                for (int v = 0; v < kWords; ++v)
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) x[v][e] = divided_anyhow(x[v][e], temp);
         }
+        T* to = out + at;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            x[v][e] = open & (1u << e) ? Store<T>::round(x[v][e]) : -INFINITY;
-            Store<T>::store(raw[v] + e, x[v][e]);
+        for (int v = 0; v < kWords; ++v) {
+            const int i = at + v * kPer * kLogitsThreads;
+            unsigned skip = left[v] >> shift & kAll;
+            if (!kWhole && i + kPer > n) skip |= i < n ? kAll << (n - i) & kAll : kAll;
+            const unsigned open = on[v] >> shift & ~skip;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                x[v][e] = open & (1u << e) ? Store<T>::round(x[v][e]) : -INFINITY;
+                Store<T>::store(raw[v] + e, x[v][e]);
+            }
+#pragma unroll
+            for (int e = 0; e < kPer; e += 2) top = max3_nan(top, x[v][e], x[v][e + 1]);
+            if (kWhole && !skip) *reinterpret_cast<uint4*>(to + v * kPer * kLogitsThreads) = *reinterpret_cast<const uint4*>(raw[v]);
+            else
+#pragma unroll
+                for (int e = 0; e < kPer; ++e)
+                    if (!(skip & (1u << e))) to[v * kPer * kLogitsThreads + e] = raw[v][e];
         }
-#pragma unroll
-        for (int e = 0; e < kPer; e += 2) top = max3_nan(top, x[v][e], x[v][e + 1]);
-        if (!skip && a.vector) *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(raw[v]);
-        else
-#pragma unroll
-            for (int e = 0; e < kPer; ++e)
-                if (!(skip & (1u << e))) out[i + e] = raw[v][e];
-    }
+    };
+    if (threadIdx.x == 0) s_where = INT_MAX;
+    if (a.vector && n == kLogitsLong) pass(std::true_type());
+    else pass(std::false_type());
     if (!a.best) return;
     const unsigned key = unsigned(argmax_key(top + 0.0f, 0) >> 32);  // + 0: a negative zero equals a positive one
     const unsigned warp_key = __reduce_max_sync(0xffffffffu, key);

@@ -373,11 +373,12 @@ template <typename K> size_t shared_marks(K kernel, const chroma_b200_pages& p) 
 // Bytes of the best of every segment of every row: of k_logits, or of k_logits_rest and k_logits_heard.
 int64_t logits_best_bytes(int64_t rows, int64_t vocab) { return rows * ((vocab + kLogitsShort - 1) / kLogitsShort + 1) * 8; }
 
-// CTAs that share a row in k_logits_heard: two a SM at once, and as many as it takes for every entry that can come to have a
-// slot, and every word of bits a place; no more than there are long segments.
+// CTAs that share a row in k_logits_heard: one a SM in all (two a SM, with half the threads each, took 33 us for 64 rows where this
+// takes 31, and 22 for twelve where this takes 16), and as many as it takes for every entry that can come to have a slot,
+// and every word of bits a place; no more than there are long segments.
 int heard_ctas(const chroma_b200_logits& g) {
     const int64_t words = (int64_t(g.vocab) + 31) / 32, come = (g.history ? int64_t(g.width) : 0) + (g.bias_ids ? g.biases : 0);
-    int64_t ctas = 2 * sm_count() / g.rows, need = (words + kHeardWords - 1) / kHeardWords;
+    int64_t ctas = sm_count() / g.rows, need = (words + kHeardWords - 1) / kHeardWords;
     if (come > kHeardMost) need = std::max(need, (words * 32 + kHeardMost - 1) / kHeardMost);
     ctas = std::max(ctas, need);
     return int(std::max<int64_t>(1, std::min(ctas, std::max(need, (words + 127) / 128))));

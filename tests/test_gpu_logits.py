@@ -157,3 +157,76 @@ def test_refusals(gpu) -> None:  # type: ignore[no-untyped-def]
     with pytest.raises(TypeError):
         call(x.tolist())
     assert call(x[:0]).shape == (0, 100)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,width,biases", [
+    (300, 33, 40, 3), (160, 4097, 7000, 300), (80, 20011, 300, 9), (75, 16384, 6000, 400), (300, 1, 2, 1), (40, 70000, 9000, 7),
+])
+def test_many_rows(gpu, dtype, rows, vocab, width, biases) -> None:  # type: ignore[no-untyped-def]
+    # So many that the entries that occurred and the others are processed by launches of their own.
+    x, more = case(rows, vocab, width, biases, dtype, vocab + rows)
+    want = ref.logits(x, **more)
+    before = x.clone()
+    got, ids = chroma_b200.process_logits(x, argmax=True, **more)
+    scale = float(x.float().abs().max()) * 2 + width + 4 * biases + 2
+    check(got, want, dtype, 2 * scale)
+    assert torch.equal(x, before)
+    np.testing.assert_array_equal(ids.cpu().numpy(), largest(got))
+    again = x.clone()
+    assert chroma_b200.process_logits(again, out=again, **more) is again
+    assert torch.equal(again, got)
+    # Rows at any address, in place.
+    wide = torch.zeros(rows, vocab + 9, dtype=dtype, device="cuda")
+    view = wide[:, 3 : 3 + vocab]
+    view.copy_(x)
+    _, same = chroma_b200.process_logits(view, out=view, argmax=True, **more)
+    assert torch.equal(view, got) and torch.equal(same, ids)
+    assert not wide[:, :3].any() and not wide[:, 3 + vocab :].any()
+
+
+@pytest.mark.parametrize("left", ["history", "bias", "mask", "temperature", "repetition", "frequency", "presence", "prompts", "all"])
+def test_any_part_may_be_missing_of_many_rows(gpu, left) -> None:  # type: ignore[no-untyped-def]
+    x, more = case(200, 5000, 60, 9, torch.float32, 12)
+    gone = {"history": ["history", "lengths", "prompts", "repetition", "presence", "frequency"],
+            "bias": ["bias", "bias_ids"], "all": list(more)}.get(left, [left])
+    more = {k: v for k, v in more.items() if k not in gone}
+    got, ids = chroma_b200.process_logits(x, argmax=True, **more)
+    check(got, ref.logits(x, **more), torch.float32, 200.0)
+    np.testing.assert_array_equal(ids.cpu().numpy(), largest(got))
+    assert torch.equal(chroma_b200.process_logits(x, **more), got)
+
+
+def test_infinities_ties_and_nan_in_many_rows(gpu) -> None:  # type: ignore[no-untyped-def]
+    x = torch.zeros(600, 9000, device="cuda").reshape(100, 6, 9000)
+    x[:, 0, 100] = x[:, 0, 5000] = 2.0
+    x[:, 1] = -float("inf")
+    x[:, 2, 300] = x[:, 2, 8999] = float("nan")
+    x[:, 3, 4000], x[:, 3, 4001] = float("inf"), -float("inf")
+    x[:, 4] = -0.0
+    x[:, 4, 8000] = 0.0
+    x[:, 5, 4095], x[:, 5, 4096] = 1.0, 1.0
+    x = x.reshape(600, 9000)
+    got, ids = chroma_b200.process_logits(x, argmax=True)
+    assert ids.reshape(100, 6).tolist() == [[100, 0, 300, 4000, 0, 4095]] * 100
+    assert torch.equal(got.nan_to_num(7.0), x.nan_to_num(7.0))
+    # The first of the equals has a bias of nothing; then the largest goes to an entry that occurred, and ties with it.
+    listed = torch.tensor([[100, 4095, 300]], dtype=torch.int32, device="cuda").expand(600, -1)
+    _, ids = chroma_b200.process_logits(x, bias_ids=listed, bias=torch.zeros(600, 3, device="cuda"), argmax=True)
+    assert ids.reshape(100, 6).tolist() == [[100, 0, 300, 4000, 0, 4095]] * 100
+    _, ids = chroma_b200.process_logits(x, bias_ids=listed, bias=torch.full((600, 3), -1.0, device="cuda"), argmax=True)
+    assert ids.reshape(100, 6).tolist() == [[5000, 0, 300, 4000, 0, 4096]] * 100
+    mask = torch.zeros(600, 282, dtype=torch.int32, device="cuda")
+    got, ids = chroma_b200.process_logits(x, mask=mask, bias_ids=listed, bias=torch.zeros(600, 3, device="cuda"), argmax=True)
+    assert bool(torch.isneginf(got).all()) and not ids.any()
+
+
+def test_biases_of_many_rows_add_up_in_list_order(gpu) -> None:  # type: ignore[no-untyped-def]
+    x = torch.zeros(300, 300, device="cuda")
+    values = torch.tensor([[1e8, 1.0, -1e8, 1.0] * 100], device="cuda").expand(300, -1)
+    for n in (80, 400):  # more than are kept in shared memory
+        want = np.float32(0)
+        for w in values[0, :n].cpu().numpy():
+            want = np.float32(want + w)
+        got = chroma_b200.process_logits(x, bias_ids=torch.full((300, n), 7, dtype=torch.int32, device="cuda"), bias=values[:, :n])
+        assert torch.equal(got[:, 7], torch.full((300,), float(want), device="cuda")) and not got[:, 8:].any()
