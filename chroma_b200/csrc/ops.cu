@@ -54,13 +54,24 @@ void check(cudaError_t status, const char* what) {
 }
 
 template <typename... Params, typename... Args>
-void launch(cudaStream_t s, dim3 grid, dim3 block, size_t smem, void (*kernel)(Params...), Args&&... args) {
+void launch_clusters(cudaStream_t s, int ctas, dim3 grid, dim3 block, size_t smem, void (*kernel)(Params...), Args&&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(ctas);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctas > 1 ? 1 : 0;
     check(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...), "kernel launch");
+}
+
+template <typename... Params, typename... Args>
+void launch(cudaStream_t s, dim3 grid, dim3 block, size_t smem, void (*kernel)(Params...), Args&&... args) {
+    launch_clusters(s, 1, grid, block, smem, kernel, std::forward<Args>(args)...);
 }
 
 // A kernel that may start while the one before it drains; it waits for that one's results itself.
@@ -275,14 +286,20 @@ void attention_fp32(const PagedArgs& a, const chroma_b200_attention& g, cudaStre
     const int64_t lines = int64_t(a.kv) * p.blocks, items = a.slots * lines;
     const int per_item = a.starts && a.group < kF32Rows ? kF32Rows / a.group : 1;
     p.whole = space.whole(a.slots, a.kv, int64_t(a.width) * a.page, a.starts);
-    const int64_t blocks = a.starts ? (int64_t(a.tokens) + per_item - 1) / per_item * lines : p.whole ? items : sm_count() * 2;
+    int64_t blocks = a.starts ? (int64_t(a.tokens) + per_item - 1) / per_item * lines : p.whole ? items : sm_count() * 2;
+    // Items of a prompt that leave SMs without work share them out, as long as every warp may have two units (16 tokens after
+    // 8,000, 16/2 heads of 64: 47 us, without 174; after 4,000 with 64/8 heads 70 and 102).
+    p.share = 1;
+    if (a.starts)
+        while (p.share < 8 && 2 * p.share * blocks <= 2 * sm_count() && int64_t(a.width) * a.page >= 2 * p.share * 2 * kF32Warps * 32) p.share *= 2;
+    blocks *= p.share;
     want(blocks < kMaxRows, "more than 2^30 heads");
     if (!p.whole) space.place(p, g);
     const auto run = [&](auto words) {
         constexpr int W = decltype(words)::value, DP = W * 4 < 32 ? 32 : W * 4;
         constexpr int smem = sizeof(F32Space<W>);
         if (smem > 48 * 1024) check(cudaFuncSetAttribute(k_paged_fp32<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "smem attribute");
-        launch(s, dim3(unsigned(blocks)), dim3(32 * kF32Warps), smem, k_paged_fp32<W>, p, per_item);
+        launch_clusters(s, p.share, dim3(unsigned(blocks)), dim3(32 * kF32Warps), smem, k_paged_fp32<W>, p, per_item);
         if (p.whole) return;
         if (a.slots >= blocks / lines / 4) launch_after(s, dim3(unsigned(blocks), 1), dim3(256), k_paged_join<float, DP, true>, p, kF32Rows);
         else launch_after(s, dim3(unsigned(blocks), kF32Rows), dim3(256), k_paged_join<float, DP, false>, p, kF32Rows);

@@ -25,6 +25,7 @@ struct PagedDecodeArgs {
     PagedArgs a;
     int blocks;      // items per key-value head
     int whole;       // one CTA per item, no cuts
+    int share;       // CTAs of a cluster that share the units of a prompt's item (fp32); 1 for tokens
     int least;       // no cut leaves a CTA fewer units than this
     int q_vector;    // query rows are 16-byte aligned
     int full;        // head rows fill the padded row

@@ -7,13 +7,14 @@
 // walks the key's row there and multiplies each 16-byte word with the same words of the 8 query rows, which all lanes read
 // from the same place, so a score needs no exchange between lanes. (Rows of 64 bytes are read by their lanes directly.)
 // Values are read with a row spread over `kWords` lanes, the 8 weights of a key in two words of shared memory. Single tokens
-// are cut, merged and joined as in paged_decode.cuh.
+// are cut, merged and joined as in paged_decode.cuh. Few items of a prompt after a long cache are each shared by the CTAs of a
+// cluster, which merge through one another's shared memory.
 //
 // What bounds it: where caches are short, the latency of five dependent reads; else shared memory and its load instructions
 // (of 32 keys and 64 values: 1,024 FMA instructions a warp, and about 400 cycles of the SM's load pipe; with each lane reading
 // its own key from global memory, and weights passed by shuffles, it was 870). 64 sequences of 500-2,000 positions with 64/8
 // heads of 64: 109 us, 12 TFLOP/s (143 in that form); two of 30,000-60,000 with 8/2 heads of 128: 78 us; two prompts of 1,000
-// with 16/4 heads of 64: 297 us. One sequence of 160 with 8 heads of 16: 7.7 us one call after another.
+// with 16/4 heads of 64: 297 us; 16 tokens after 8,000, 16/2 heads of 64: 47 us. One sequence of 160 with 8 heads of 16: 7.7 us one call after another.
 #pragma once
 
 #include <limits.h>
@@ -44,6 +45,13 @@ template <int kWords> struct F32Space {
     F32Row rows[kF32Rows];
 };
 
+// The float at the same place of shared memory in a CTA of the cluster.
+__device__ __forceinline__ float mate_value(const float* p, int rank) {
+    float x;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(cluster_addr(p, uint32_t(rank))) : "memory");
+    return x;
+}
+
 // kWords: 16-byte words of a head's row, rounded up to 4, 8, 16 or 32.
 template <int kWords> __global__ void __launch_bounds__(32 * kF32Warps, 2) k_paged_fp32(const __grid_constant__ PagedDecodeArgs p, int tokens_per_item) {
     constexpr int U = 32, R = kF32Rows, kAt = 32 / kWords, DP = kWords * 4 < 32 ? 32 : kWords * 4;
@@ -57,10 +65,11 @@ template <int kWords> __global__ void __launch_bounds__(32 * kF32Warps, 2) k_pag
 
     // ---- what this CTA has: tokens of a prompt, or a part of the line of single tokens
     const bool prompt = a.starts;
-    const int items = a.kv * p.blocks, item = blockIdx.x % items, kvh = item / p.blocks, block = item % p.blocks;
+    const int share = p.share, mate = share > 1 ? blockIdx.x % share : 0, mates_block = share > 1 ? blockIdx.x / share : blockIdx.x;
+    const int items = a.kv * p.blocks, item = mates_block % items, kvh = item / p.blocks, block = item % p.blocks;
     LinePart<U> part{};
     int token0 = 0;
-    if (prompt) token0 = int(blockIdx.x) / items * tokens_per_item;
+    if (prompt) token0 = mates_block / items * tokens_per_item;
     else part = cut_line<U, kF32Warps>(p);
     LinePart<U> at = part;
     int4 join = make_int4(0, 0, 0, 0);
@@ -129,7 +138,7 @@ template <int kWords> __global__ void __launch_bounds__(32 * kF32Warps, 2) k_pag
             if (at.u >= seen.units) at.next_slot(a);
         }
 
-        // ---- its units, 8 warps in turn
+        // ---- its units, 8 warps of each CTA in turn
         float m[R], l[R], o[R][4];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -138,7 +147,7 @@ template <int kWords> __global__ void __launch_bounds__(32 * kF32Warps, 2) k_pag
 #pragma unroll
             for (int c = 0; c < 4; ++c) o[r][c] = 0.f;
         }
-        for (int u = first + warp; u < last; u += kF32Warps) {
+        for (int u = first + mate * kF32Warps + warp; u < last; u += share * kF32Warps) {
             const int j = seen.begin(u) + lane, entry = int(a.by_page.div(uint32_t(j))), row = j - entry * a.page;
             int id = j <= seen.pos && entry < a.width ? __ldg(a.table + slot * a.ts + entry) : -1;
             if (id >= a.pages) id = -1;
@@ -242,19 +251,33 @@ template <int kWords> __global__ void __launch_bounds__(32 * kF32Warps, 2) k_pag
 #pragma unroll
             for (int r = 0; r < R; ++r) sm.warp_ml[warp][r] = make_float2(m[r], l[r]);
         __syncthreads();
-        for (int e = threadIdx.x; e < R * kWords * 4; e += 32 * kF32Warps) {
+        if (share > 1) cluster_sync_all();
+        for (int e = threadIdx.x + mate * 32 * kF32Warps; e < R * kWords * 4; e += share * 32 * kF32Warps) {
             const int r = e / (kWords * 4), d = e % (kWords * 4);
             const F32Row row = sm.rows[r];
             if (d >= a.dim || row.token < 0 || row.slot != slot) continue;
             float top = -INFINITY, sum = 0.f, x = 0.f;
+            if (share > 1) {  // the warps of all CTAs, in their order
+                for (int c = 0; c < share; ++c)
 #pragma unroll
-            for (int v = 0; v < kF32Warps; ++v) top = fmaxf(top, sm.warp_ml[v][r].x);
+                    for (int v = 0; v < kF32Warps; ++v) top = fmaxf(top, mate_value(&sm.warp_ml[v][r].x, c));
+                for (int c = 0; c < share; ++c)
 #pragma unroll
-            for (int v = 0; v < kF32Warps; ++v) {
-                const float2 ml = sm.warp_ml[v][r];
-                const float weight = part_weight(ml.x, ml.y, top);
-                sum += ml.y * weight;
-                x += sm.warps[v].merge[r][d] * weight;
+                    for (int v = 0; v < kF32Warps; ++v) {
+                        const float total = mate_value(&sm.warp_ml[v][r].y, c), weight = part_weight(mate_value(&sm.warp_ml[v][r].x, c), total, top);
+                        sum += total * weight;
+                        x += mate_value(&sm.warps[v].merge[r][d], c) * weight;
+                    }
+            } else {
+#pragma unroll
+                for (int v = 0; v < kF32Warps; ++v) top = fmaxf(top, sm.warp_ml[v][r].x);
+#pragma unroll
+                for (int v = 0; v < kF32Warps; ++v) {
+                    const float2 ml = sm.warp_ml[v][r];
+                    const float weight = part_weight(ml.x, ml.y, top);
+                    sum += ml.y * weight;
+                    x += sm.warps[v].merge[r][d] * weight;
+                }
             }
             if (complete) {
                 const HeadEnd he = head_end(top, sum, sink_log2<float>(a.sinks, a.sinks_fp32, row.head));
@@ -267,6 +290,7 @@ template <int kWords> __global__ void __launch_bounds__(32 * kF32Warps, 2) k_pag
             }
         }
         __syncthreads();
+        if (share > 1) cluster_sync_all();
     }
     if (!prompt && !p.whole && threadIdx.x == 0) p.joins[blockIdx.x] = join;
 }

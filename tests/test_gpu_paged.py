@@ -441,3 +441,21 @@ def test_refusals(gpu) -> None:  # type: ignore[no-untyped-def]
     empty = call(q[:0], k, v, table, n, torch.zeros(3, dtype=torch.int32).cuda())
     assert empty.shape == (0, 8, 64)
     check(call(q, k, v, table, n), ref.attention(q, k, v, table, n, scale=0.125), dtype=B16, dim=64)
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,window,first,sinks", [
+    (8, 1, 64, 16, 0, 0, True), (8, 2, 128, 48, 0, 0, False), (6, 2, 80, 5, 3000, 300, True), (16, 1, 16, 64, 200, 0, False),
+    (3, 1, 20, 32, 0, 0, True),
+])
+def test_shared_items_of_fp32_prompts(gpu, heads, kv, dim, page, window, first, sinks) -> None:  # type: ignore[no-untyped-def]
+    # Few rows and many keys: CTAs of a cluster share each item. Items with tokens of several slots among them.
+    new, prior = [5, 0, 10, 1], [7001, 300, 2500, 0]
+    k, v, table, n = cache([a + b for a, b in zip(new, prior)], dtype=F32, kv=kv, dim=dim, page=page)
+    starts = torch.tensor(np.concatenate([[0], np.cumsum(new)]), dtype=torch.int32).cuda()
+    q = queries(sum(new), heads, dim, F32)
+    s = sink_values(heads, F32) if sinks else None
+    n[3] = 0  # a token that is at no position
+    want = ref.attention(q, k, v, table, n, starts, scale=dim**-0.5, window=window, first=first, sinks=s)
+    got, logs = chroma_b200.paged_attention(q, k, v, table, n, starts, window=window, first=first, sinks=s, lse=True)
+    check(got, want, dtype=F32, dim=dim, lse=logs)
+    assert torch.equal(chroma_b200.paged_attention(q, k, v, table, n, starts, window=window, first=first, sinks=s), got)
