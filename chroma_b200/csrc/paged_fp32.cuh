@@ -14,7 +14,8 @@
 // (of 32 keys and 64 values: 1,024 FMA instructions a warp, and about 400 cycles of the SM's load pipe; with each lane reading
 // its own key from global memory, and weights passed by shuffles, it was 870). 64 sequences of 500-2,000 positions with 64/8
 // heads of 64: 109 us, 12 TFLOP/s (143 in that form); two of 30,000-60,000 with 8/2 heads of 128: 78 us; two prompts of 1,000
-// with 16/4 heads of 64: 297 us; 16 tokens after 8,000, 16/2 heads of 64: 47 us. One sequence of 160 with 8 heads of 16: 7.7 us one call after another.
+// with 16/4 heads of 64: 297 us; 16 tokens after 8,000, 16/2 heads of 64: 47 us. One sequence of 160 with 8 heads of 16:
+// 7.7 us one call after another.
 #pragma once
 
 #include <limits.h>
