@@ -387,12 +387,13 @@ k_paged_decode(PagedDecodeArgs p) {
         const int pos = next.seen.pos;
         if (fast) {
             const char* v = vlane + p.vp * next_id + p.vr * next_row;
+            const bool ok = DP >= 64 || g * 8 < DP;  // a row of 32 values ends after the words of half of the lanes
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                vw[d][0] = load_word(v + d * 128);
-                vw[d][1] = load_word(v + v1 + d * 128);
-                vw[d][2] = load_word(v + v8 + d * 128);
-                vw[d][3] = load_word(v + v8 + v1 + d * 128);
+                vw[d][0] = load_word_if(v + d * 128, ok);
+                vw[d][1] = load_word_if(v + v1 + d * 128, ok);
+                vw[d][2] = load_word_if(v + v8 + d * 128, ok);
+                vw[d][3] = load_word_if(v + v8 + v1 + d * 128, ok);
             }
         } else {
 #pragma unroll
