@@ -313,10 +313,10 @@ void attention_fp32(const PagedArgs& a, const chroma_b200_attention& g, cudaStre
 // How prompts are laid out, and their workspace: partial results of every split of every item.
 struct PromptSpace {
     int64_t items, parts = 0, bytes = 0;  // items: at least as many as there are
-    int splits = 1;
+    int tiles, splits = 1;                // tiles: pairs of tiles of rows, an item for each key-value head
     PromptSpace(int tokens, int group, int slots, int kv, int dim, int64_t positions) {
-        items = (int64_t(tokens) * group / 256 + (slots < tokens ? slots : tokens)) * kv;
-        if (items < 1) items = 1;
+        tiles = int(int64_t(tokens) * group / 256) + std::max(1, std::min(slots, tokens));
+        items = int64_t(tiles) * kv;
         // Fewer items than half the SMs share the SMs out, as long as four key tiles are left to each split.
         const int64_t most = positions / (4 * kPrTile), share = sm_count() / items;
         if (share > 1 && most > 1) splits = int(share < most ? share : most);
@@ -340,6 +340,7 @@ template <int H> void prompt_bf16(PagedPromptArgs& p, const chroma_b200_attentio
     const cuuint32_t box[3] = {64, cuuint32_t(a.group), cuuint32_t(kPrTile / (a.group <= kPrTile ? a.group : kPrTile))};
     p.q_box = kPrTile % a.group == 0 && bf16_map(&qmap, a.q, 3, dims, strides, box);
     const PromptSpace space(a.tokens, a.group, a.slots, a.kv, a.dim, int64_t(a.width) * a.page);
+    p.tiles = space.tiles;
     p.splits = space.splits;
     p.by_splits = FastDiv(uint32_t(p.splits));
     if (p.splits > 1) {

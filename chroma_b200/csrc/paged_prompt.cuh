@@ -104,6 +104,7 @@ struct PagedPromptArgs {
     int box;                 // rows of a TMA box; 0: row by row
     int q_vector, out_vector;  // rows are 16-byte aligned
     int q_box;               // Q tiles come as one TMA box: `group` heads of 128 / group tokens
+    int tiles;               // pairs of tiles of rows at most: what the workspace has room for
     int splits;              // of the keys of an item, where there are few items
     FastDiv by_splits;
     float* parts;            // [items][splits][256 rows][64 H]: what the splits of a row come to, unless there is one
@@ -141,6 +142,13 @@ struct PromptCursor {
     static __device__ __forceinline__ int rows_of(const PagedArgs& a, int s) {
         const int t0 = min(max(a.starts[s], 0), a.tokens), t1 = min(max(a.starts[s + 1], 0), a.tokens);
         return max(0, t1 - t0) * a.group;
+    }
+    // Adds up the pairs of tiles of all slots. Rows that a falling `starts` gives to several slots are counted for each, so the
+    // sum may pass what the host made room for: callers cut it there.
+    static __device__ __forceinline__ void count_tiles(const PagedArgs& a, unsigned long long* sum) {
+        unsigned long long mine = 0;
+        for (int s = threadIdx.x; s < a.slots; s += blockDim.x) mine += (rows_of(a, s) + 255) / 256;
+        if (mine) atomicAdd(sum, mine);
     }
     __device__ __forceinline__ bool next(const PagedPromptArgs& p, int total, PromptItem& w) {
         const unsigned i = unsigned(round) * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
@@ -276,7 +284,8 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
     uint32_t* gone = reinterpret_cast<uint32_t*>(KV + kStages * Shape::kStage);  // [kStages][4]
     __shared__ uint64_t q_full[2], q_empty[2], kv_full[kStages], kv_empty[kStages], s_full[2], s_free[2], p_full[2], o_done[2];
     __shared__ uint32_t tmem_base;
-    __shared__ int s_total, tile_counts[kPrSortedSlots];
+    __shared__ int tile_counts[kPrSortedSlots];
+    __shared__ unsigned long long s_total;
     __shared__ volatile int abort_flag;
     const PagedArgs& a = p.a;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -305,21 +314,17 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    {
-        int mine = 0;
-        for (int s = threadIdx.x; s < a.slots; s += kPrThreads) mine += (PromptCursor::rows_of(a, s) + 255) / 256;
-        if (mine) atomicAdd(&s_total, mine);
-    }
+    PromptCursor::count_tiles(a, &s_total);
     __syncthreads();
-    const int total = s_total;
+    const int total = int(min(s_total, (unsigned long long)p.tiles));
     const uint32_t tmem = tmem_base;
     // With few sequences their tiles are put in order, the later (with more keys before them) first, whatever the sequence:
     // four prompts of 2,048 tokens are then within 1% of an even load, against 10% in the order of the sequences.
-    const bool sorted = p.splits == 1 && total <= kPrSorted && a.slots <= kPrSortedSlots;
+    const bool sorted = p.splits == 1 && s_total <= kPrSorted && a.slots <= kPrSortedSlots;
     if (sorted) {
         for (int s = threadIdx.x; s < a.slots; s += kPrThreads) tile_counts[s] = (PromptCursor::rows_of(a, s) + 255) / 256;
         __syncthreads();
-        for (int e = threadIdx.x; e < total; e += kPrThreads) {
+        for (int e = threadIdx.x; e < int(s_total); e += kPrThreads) {
             int slot = 0, tile = e, place = 0;
             while (tile >= tile_counts[slot]) tile -= tile_counts[slot++];
             for (int s = 0; s < a.slots; ++s) place += max(0, tile_counts[s] - 1 - tile) + (s < slot && tile_counts[s] > tile);
@@ -696,17 +701,15 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
 // computed again.
 template <int H> __global__ void __launch_bounds__(256) k_prompt_join(const __grid_constant__ PagedPromptArgs p) {
     constexpr int D = 64 * H;
-    __shared__ int s_total;
+    __shared__ unsigned long long s_total;
     const PagedArgs& a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) s_total = 0;
     __syncthreads();
-    int mine = 0;
-    for (int s = threadIdx.x; s < a.slots; s += 256) mine += (PromptCursor::rows_of(a, s) + 255) / 256;
-    if (mine) atomicAdd(&s_total, mine);
+    PromptCursor::count_tiles(a, &s_total);
     __syncthreads();
     const unsigned i = blockIdx.x >> 3;
-    if (i >= unsigned(s_total) * unsigned(a.kv)) return;
+    if (i >= unsigned(min(s_total, (unsigned long long)p.tiles)) * unsigned(a.kv)) return;
     PromptCursor cursor(a);
     PromptItem w;
     cursor.find(p, i, w);
