@@ -54,7 +54,8 @@ def paged_append(keys: Tensor, values: Tensor, new_keys: Tensor, new_values: Ten
 
     Rows ``starts[b] : starts[b + 1]`` are slot b's (``starts`` int32 ``[slots + 1]``, from 0 to ``tokens``; without it
     there is one row per slot). ``lengths`` counts them already: the last is written at ``lengths[b] - 1``. The pages
-    must belong to the slot alone from there on (``step_pages`` sees to it); rows without a page are dropped.
+    must belong to the slot alone from there on (``step_pages`` sees to it); rows without a page, those past the end of
+    the table among them, are dropped.
     """
     ops.paged_append(keys, values, new_keys, new_values, table, lengths, starts)
 

@@ -42,11 +42,14 @@ struct PagedArgs {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// Length of a slot: one past its last token's position, which may lie past what its table can name.
+__device__ __forceinline__ int length_of(const int* lengths, int slot) { return max(lengths[slot], 0); }
+
 // Rows a slot holds, within what its table can name.
 __device__ __forceinline__ int held_rows(const int* lengths, int slot, int width, int page) {
     const int64_t most = int64_t(width) * page;
-    const int n = lengths[slot];
-    return n < 0 ? 0 : int64_t(n) > most ? int(most) : n;
+    const int n = length_of(lengths, slot);
+    return int64_t(n) > most ? int(most) : n;
 }
 
 // Slot of a token: the last slot whose first row is not after it, or -1 (rows before the first slot or past the last).
@@ -117,10 +120,10 @@ template <typename T> __global__ void __launch_bounds__(32 * kAppendWarps) k_pag
         int found = -1;
 #pragma unroll 4
         for (int s = lane; s < a.slots; s += 32) {
-            const int first = a.starts[s], end = a.starts[s + 1], held = held_rows(a.lengths, s, a.width, a.page);
+            const int first = a.starts[s], end = a.starts[s + 1], length = length_of(a.lengths, s);
             if (first <= token && token < end) {
                 found = s;
-                pos = held - end + token;
+                pos = length - end + token;
             }
         }
         const unsigned who = __ballot_sync(0xffffffffu, found >= 0);
@@ -130,10 +133,12 @@ template <typename T> __global__ void __launch_bounds__(32 * kAppendWarps) k_pag
     } else {
         if (a.starts) slot = slot_of(a.starts, a.slots, token);
         if (slot < 0) return;
-        pos = held_rows(a.lengths, slot, a.width, a.page) - (a.starts ? a.starts[slot + 1] - token : 1);
+        pos = length_of(a.lengths, slot) - (a.starts ? a.starts[slot + 1] - token : 1);
     }
     if (pos < 0) return;
-    const int entry = int(a.by_page.div(uint32_t(pos))), id = a.table[slot * a.ts + entry];
+    const int entry = int(a.by_page.div(uint32_t(pos)));
+    if (entry >= a.width) return;
+    const int id = a.table[slot * a.ts + entry];
     if (id < 0 || id >= a.pages) return;
     T* k = static_cast<T*>(a.k) + id * a.kp + (pos - entry * a.page) * a.kr;
     T* v = static_cast<T*>(a.v) + id * a.vp + (pos - entry * a.page) * a.vr;

@@ -37,21 +37,25 @@ struct PagedDecodeArgs {
     unsigned* error;
 };
 
-// What a token at the end of a slot sees, in units of U positions: pre units from 0, then those from main0 on.
+// What a token at the end of a slot sees, in units of U positions: pre units from 0, then those from main0 on, as far as
+// the table goes.
 template <int U> struct SeenUnits {
     int pos = -1, pre = 0, main0 = 0, units = 1;  // a slot with nothing to see has one unit with no visible key
     __device__ SeenUnits() {}
     __device__ SeenUnits(const PagedArgs& a, int slot) {
-        const int last = held_rows(a.lengths, slot, a.width, a.page) - 1;
+        const int last = length_of(a.lengths, slot) - 1;
         if (last >= 0) set(a, last, last);
     }
     __device__ __forceinline__ void set(const PagedArgs& a, int at, int last) {  // tokens at positions at .. last
         pos = last;
-        const int low = a.window > 0 ? max(0, at - a.window + 1) : 0;
-        pre = (min(a.first, low) + U - 1) / U;
+        const int low = a.window > 0 ? max(0, at - a.window + 1) : 0, top = min(last, a.width * a.page - 1);
+        pre = (min(a.first, min(low, top + 1)) + U - 1) / U;
         main0 = max(low / U, pre);
-        units = pre + pos / U - main0 + 1;
-        if (units < 1) units = 1;
+        units = pre + max(0, top / U - main0 + 1);
+        if (units < 1) {  // the window lies past the table
+            units = 1;
+            main0 = top / U;
+        }
     }
     __device__ __forceinline__ int begin(int u) const { return (u < pre ? u : main0 + u - pre) * U; }
 };

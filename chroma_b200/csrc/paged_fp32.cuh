@@ -90,7 +90,7 @@ template <int kWords> __global__ void __launch_bounds__(32 * kF32Warps, 2) k_pag
                     row.head = kvh * a.group + block * R + threadIdx.x % per;
                     if (row.slot >= 0) {
                         row.token = token;
-                        row.pos = held_rows(a.lengths, row.slot, a.width, a.page) - (prompt ? a.starts[row.slot + 1] - token : 1);
+                        row.pos = length_of(a.lengths, row.slot) - (prompt ? a.starts[row.slot + 1] - token : 1);
                     }
                 }
                 sm.rows[threadIdx.x] = row;

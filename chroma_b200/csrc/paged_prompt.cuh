@@ -188,13 +188,13 @@ struct PromptCursor {
         w.slot = slot;
         w.rows = rows;
         w.token0 = min(max(a.starts[slot], 0), a.tokens);
-        w.pos0 = held_rows(a.lengths, slot, a.width, a.page) - rows / a.group;
+        w.pos0 = length_of(a.lengths, slot) - rows / a.group;
         w.active = w.row0 + kPrTile < rows ? 2 : 1;
         const int first = w.pos0 + int(p.by_group.div(w.row0)), last = w.pos0 + int(p.by_group.div(min(w.row0 + 256, rows) - 1));
-        const int low = a.window > 0 ? max(0, first - a.window + 1) : 0;
-        w.pre = (min(a.first, low) + kPrTile - 1) / kPrTile;
+        const int low = a.window > 0 ? max(0, first - a.window + 1) : 0, top = min(last, a.width * a.page - 1);
+        w.pre = (min(a.first, min(low, top + 1)) + kPrTile - 1) / kPrTile;
         w.main0 = max(low / kPrTile, w.pre);
-        w.tiles = last < 0 ? 0 : w.pre + max(0, last / kPrTile - w.main0 + 1);
+        w.tiles = last < 0 ? 0 : w.pre + max(0, top / kPrTile - w.main0 + 1);
         w.skip = 0;
         w.part = 0;
     }
@@ -211,8 +211,9 @@ __device__ __noinline__ void attend_row(const PagedArgs& a, int token, int head,
 #pragma unroll
     for (int c = 0; c < 4; ++c) o[c] = 0.f;
     const int low = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    const int first = min(a.first, low);  // [0, first) then [low, pos]
-    const int total = max(0, pos + 1 - low + first);
+    const int top = min(pos, a.width * a.page - 1);
+    const int first = min(a.first, min(low, top + 1));  // [0, first) then [low, top]
+    const int total = first + max(0, top + 1 - low);
     for (int base = 0; base < total; base += 32) {
         const int i = base + lane;
         const int j = i < first ? i : low + i - first;

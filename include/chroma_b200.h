@@ -254,7 +254,8 @@ typedef struct chroma_b200_pages {
  * 16-byte aligned. */
 
 /* Writes new rows into the pages that already belong to their sequences: row i of slot b (rows starts[b] to
- * starts[b + 1]; row b alone where `starts` is NULL) goes to position lengths[b] - rows + i. Layer 0 of the pools.
+ * starts[b + 1]; row b alone where `starts` is NULL) goes to position lengths[b] - rows + i; rows whose position has no
+ * page, or lies past the table, are dropped. Layer 0 of the pools.
  * new_strides: elements between tokens and heads of new_keys, then of new_values. */
 int chroma_b200_paged_append(const chroma_b200_pages* pages, const void* new_keys, const void* new_values,
                              const int64_t* new_strides, const int32_t* starts, int32_t tokens, void* stream, char* err,
@@ -277,7 +278,7 @@ typedef struct chroma_b200_attention {
 } chroma_b200_attention;
 
 /* out = softmax(scale q.K^T) V of each token over the positions it sees. Token i of slot b is at position
- * p = lengths[b] - tokens of b + i and sees j <= p with p - j < window or j < first. The attention of
+ * p = lengths[b] - tokens of b + i (which may lie past the table) and sees j <= p with p - j < window or j < first. The attention of
  * chroma/models/gpt_oss.py:133-151 (learned sinks, sliding window) over pages; `lse` is the logarithm of the sum. A
  * token that sees nothing gives zeros, and its sink (or -inf) as lse. */
 int chroma_b200_paged_attention(const chroma_b200_pages* pages, const chroma_b200_attention* args, void* stream,

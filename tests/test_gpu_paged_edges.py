@@ -76,3 +76,73 @@ def test_falling_starts_stay_within_the_workspace(gpu) -> None:  # type: ignore[
     rise = torch.arange(slots + 1, dtype=torch.int32).cuda() * (tokens // slots)
     want = ref.attention(q, k, v, table, n, rise, scale=0.125)
     check(chroma_b200.paged_attention(q, k, v, table, n, rise), want, dtype=B16, dim=64)
+
+
+# ---- lengths past the end of the table: such positions have no page, and move no other
+
+@pytest.mark.parametrize("dtype,kv,dim,page", [(B16, 8, 64, 64), (F32, 1, 16, 5), (B16, 3, 8, 1)])
+@pytest.mark.parametrize("slots", [6, 300])
+def test_rows_past_the_table_are_dropped(gpu, dtype, kv, dim, page, slots) -> None:  # type: ignore[no-untyped-def]
+    end = 2 * page  # positions of a slot
+    k, v, table, _ = cache([end] * slots, dtype=dtype, kv=kv, dim=dim, page=page, width=2, spare=0)
+    new = [(2, 1, 3, 0, 1, 4)[s % 6] for s in range(slots)]
+    lengths = [(end, end + 1, end + 2, end + 9, 2**31 - 1, end + 5)[s % 6] for s in range(slots)]
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    starts = torch.tensor([sum(new[:s]) for s in range(slots + 1)], dtype=torch.int32).cuda()
+    rows = torch.randn(sum(new), 2 * kv, dim, device="cuda").to(dtype)
+    for given in (starts, None):
+        nk, nv = (rows[:, :kv], rows[:, kv:]) if given is not None else (rows[:slots, :kv], rows[:slots, kv:])
+        want_k, want_v = k.clone(), v.clone()
+        at = 0
+        for s in range(slots):
+            count = new[s] if given is not None else 1
+            for i in range(count):
+                p = lengths[s] - count + i
+                if p < end:
+                    want_k[table[s, p // page], p % page], want_v[table[s, p // page], p % page] = nk[at + i], nv[at + i]
+            at += count
+        got_k, got_v = k.clone(), v.clone()
+        chroma_b200.paged_append(got_k, got_v, nk, nv, table, n, given)
+        assert torch.equal(got_k, want_k) and torch.equal(got_v, want_v)
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,page", [
+    (F32, 8, 1, 16, 7), (F32, 4, 2, 64, 16), (B16, 16, 2, 64, 16), (B16, 8, 8, 128, 48), (B16, 6, 2, 80, 24),
+    (B16, 4, 1, 32, 5), (B16, 64, 8, 64, 64),
+])
+@pytest.mark.parametrize("window,first", [(0, 0), (10, 0), (40, 3), (40, 500), (3, 20)])
+@pytest.mark.parametrize("prompt", [False, True])
+def test_tokens_past_the_table_are_at_their_positions(gpu, dtype, heads, kv, dim, page, window, first, prompt) -> None:  # type: ignore[no-untyped-def]
+    end = 4 * page
+    k, v, table, _ = cache([end] * 6, dtype=dtype, kv=kv, dim=dim, page=page, width=4, spare=0)
+    lengths, new = [end + 3, end - 1, end + 30, end + 12, end + 700, end], [5, 3, 70, 12, 1, 9]
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    starts = torch.tensor([sum(new[:s]) for s in range(7)], dtype=torch.int32).cuda() if prompt else None
+    q = queries(sum(new) if prompt else 6, heads, dim, dtype)
+    s = sink_values(heads, F32)
+    # the same in a table that is wide enough to name those positions, and names no page there
+    wide = torch.cat([table, torch.full((6, 700 // page + 1), -1, dtype=torch.int32, device="cuda")], 1)
+    want = ref.attention(q, k, v, wide, n, starts, scale=0.2, window=window, first=first, sinks=s)
+    got, logs = chroma_b200.paged_attention(q, k, v, table, n, starts, scale=0.2, window=window, first=first, sinks=s, lse=True)
+    check(got, want, dtype=dtype, dim=dim, lse=logs)
+    # a length as large as there are: what is left is the first tokens, or everything where there is no window
+    n.fill_(2**31 - 1)
+    seen = torch.full_like(n, min(first, end) if window else end)
+    want = ref.attention(q[:6], k, v, table, seen, scale=0.2, sinks=s)
+    far = torch.arange(7, dtype=torch.int32).cuda() if prompt else None
+    got = chroma_b200.paged_attention(q[:6], k, v, table, n, far, scale=0.2, window=window, first=first, sinks=s)
+    check(got, want, dtype=dtype, dim=dim)
+
+
+def test_long_caches_past_the_table(gpu) -> None:  # type: ignore[no-untyped-def]
+    # Cut and joined, or split; the tokens lie in the window's reach behind the end.
+    for dtype, dim, heads in ((B16, 64, 16), (B16, 128, 8), (F32, 64, 8)):
+        k, v, table, _ = cache([4096, 4096], dtype=dtype, kv=2, dim=dim, page=16, width=256)
+        wide = torch.cat([table, torch.full((2, 64), -1, dtype=torch.int32, device="cuda")], 1)
+        n = torch.tensor([4096 + 500, 4096 + 20], dtype=torch.int32).cuda()
+        for starts in (None, torch.tensor([0, 3, 23], dtype=torch.int32).cuda()):
+            q = queries(23 if starts is not None else 2, heads, dim, dtype)
+            for window in (0, 3000, 400):
+                want = ref.attention(q, k, v, wide, n, starts, scale=0.2, window=window, first=window // 300)
+                got, logs = chroma_b200.paged_attention(q, k, v, table, n, starts, scale=0.2, window=window, first=window // 300, lse=True)
+                check(got, want, dtype=dtype, dim=dim, lse=logs)
