@@ -108,6 +108,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "chroma_b200_paged_attention": (ctypes.c_int, [_VP, _VP, _VP, _CP, _SZ]),
     "chroma_b200_attention_workspace": (ctypes.c_int64, [_VP, _VP]),
     "chroma_b200_step_pages": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_int64, _VP, _CP, _SZ]),
+    "chroma_b200_step_pages_uncut": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_int64, _VP, _CP, _SZ]),
     "chroma_b200_compact_pages": (ctypes.c_int, [_VP, _VP, _VP, _VP, ctypes.c_int64, _VP, _CP, _SZ]),
     "chroma_b200_pages_workspace": (ctypes.c_int64, [_I32, _I32]),
     "chroma_b200_process_logits": (ctypes.c_int, [_VP, _VP, _CP, _SZ]),

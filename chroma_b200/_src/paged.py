@@ -6,7 +6,8 @@ A cache is two pools ``keys`` and ``values`` of pages, ``[pages, page_rows, kv_h
 sequence (below 0: none); and int32 ``lengths [slots]``, the rows that each holds. Position ``p`` of slot ``s`` is row
 ``p % page_rows`` of page ``table[s, p // page_rows]``. A step of a program that serves from it::
 
-    table, lengths, info = step_pages(table, lengths, parents, counts, keys, values)   # fork, empty, reserve
+    # fork, empty, reserve
+    table, lengths, info = step_pages(table, lengths, parents, counts, keys, values, cut=False)
     for layer in range(layers):
         ...
         paged_append(keys[layer], values[layer], k, v, table, lengths, starts)
@@ -28,8 +29,8 @@ from torch import Tensor
 
 from chroma_b200._src import native as nat
 
-_ENTRIES = ("paged_append", "paged_attention", "attention_workspace", "step_pages", "compact_pages", "pages_workspace",
-            "process_logits", "logits_workspace")
+_ENTRIES = ("paged_append", "paged_attention", "attention_workspace", "step_pages", "step_pages_uncut", "compact_pages",
+            "pages_workspace", "process_logits", "logits_workspace")
 
 
 def _module() -> Any:
@@ -80,8 +81,8 @@ def paged_attention(q: Tensor, keys: Tensor, values: Tensor, table: Tensor, leng
     return ops.paged_attention(q, keys, values, table, lengths, starts, scale, window, first, sinks, lse, out)
 
 
-def step_pages(table: Tensor, lengths: Tensor, parents: Tensor, counts: Tensor, keys: Tensor,
-               values: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+def step_pages(table: Tensor, lengths: Tensor, parents: Tensor, counts: Tensor, keys: Tensor, values: Tensor, *,
+               cut: bool = True) -> tuple[Tensor, Tensor, Tensor]:
     """One step of a set of sequences: returns the new ``(table, lengths, info)`` and leaves the given ones as they are.
 
     Slot s continues slot ``parents[s]`` (int32 ``[slots]``: s itself, another that several slots may continue, or -1,
@@ -91,8 +92,14 @@ def step_pages(table: Tensor, lengths: Tensor, parents: Tensor, counts: Tensor, 
     slot holds is free; free pages are given out from the lowest number to slots from the lowest. ``info`` (int32,
     on the device) is [pages left free, pages short, pages copied]; where pages are short, entries stay -1, nothing is
     copied, and the step can be tried again from the old table.
+
+    A sequence may ask for rows past the end of its row of the table, ``width * page_rows`` positions. With ``cut`` its
+    length ends there, and the caller must not append the rows that were cut off: ``paged_append`` counts back from the
+    length, so it would put them over the last rows before the end. With ``cut=False`` lengths count every row that was
+    asked for; ``paged_append`` drops those past the end, ``paged_attention`` sees what has pages, and a length above
+    ``width * page_rows`` says that the sequence has outgrown its table.
     """
-    return ops.step_pages(table, lengths, parents, counts, keys, values)
+    return ops.step_pages(table, lengths, parents, counts, keys, values, cut)
 
 
 def compact_pages(table: Tensor, lengths: Tensor, keys: Tensor, values: Tensor) -> tuple[Tensor, Tensor]:

@@ -404,6 +404,30 @@ int heard_ctas(const chroma_b200_logits& g) {
 
 dim3 table_grid(const chroma_b200_pages& p) { return dim3(unsigned((p.width + 255) / 256), unsigned(p.slots)); }
 
+void step_pages(const chroma_b200_pages* p, const int32_t* parents, const int32_t* counts, int32_t* new_table, int32_t* new_lengths,
+                int32_t* info, void* workspace, int64_t workspace_bytes, bool cut, cudaStream_t s) {
+    check_pages(p);
+    want(parents && counts && new_table && new_lengths && info && workspace, "null argument");
+    want(workspace_bytes >= chroma_b200_pages_workspace(p->pages, p->slots), "workspace too small");
+    want((int64_t(p->page_rows) + 1) * p->slots < (int64_t(1) << 32), "page_rows * slots must be below 2^32");
+    want(p->slots <= 65535, "at most 65,535 slots");
+    StepArgs a{};
+    a.table = p->table, a.ts = p->table_stride, a.lengths = p->lengths, a.parents = parents, a.counts = counts;
+    a.new_table = new_table, a.new_lengths = new_lengths, a.info = info;
+    a.keeper = static_cast<unsigned*>(workspace);
+    a.free_list = static_cast<int*>(workspace) + p->pages;
+    a.copies = a.free_list + p->pages;
+    a.slots = p->slots, a.width = p->width, a.pages = p->pages, a.page = p->page_rows;
+    a.cut = cut;
+    if (one_cta(*p)) launch(s, dim3(1), dim3(1024), shared_marks(k_pages_step, *p), k_pages_step, a);
+    else {
+        check(cudaMemsetAsync(a.keeper, 0, size_t(p->pages) * 4, s), "memset");
+        launch(s, table_grid(*p), dim3(256), 0, k_pages_gather, a);
+        launch(s, dim3(1), dim3(1024), 0, k_pages_assign, a);
+    }
+    copy_pages(*p, a.copies, a.copies + 3 * p->slots, s);
+}
+
 }  // namespace
 
 extern "C" {
@@ -498,28 +522,13 @@ int64_t chroma_b200_pages_workspace(int32_t pages, int32_t slots) {
 int chroma_b200_step_pages(const chroma_b200_pages* p, const int32_t* parents, const int32_t* counts, int32_t* new_table,
                            int32_t* new_lengths, int32_t* info, void* workspace, int64_t workspace_bytes, void* stream,
                            char* err, size_t err_len) {
-    return guarded_op(err, err_len, [&] {
-        check_pages(p);
-        want(parents && counts && new_table && new_lengths && info && workspace, "null argument");
-        want(workspace_bytes >= chroma_b200_pages_workspace(p->pages, p->slots), "workspace too small");
-        want((int64_t(p->page_rows) + 1) * p->slots < (int64_t(1) << 32), "page_rows * slots must be below 2^32");
-        want(p->slots <= 65535, "at most 65,535 slots");
-        const auto s = cudaStream_t(stream);
-        StepArgs a{};
-        a.table = p->table, a.ts = p->table_stride, a.lengths = p->lengths, a.parents = parents, a.counts = counts;
-        a.new_table = new_table, a.new_lengths = new_lengths, a.info = info;
-        a.keeper = static_cast<unsigned*>(workspace);
-        a.free_list = static_cast<int*>(workspace) + p->pages;
-        a.copies = a.free_list + p->pages;
-        a.slots = p->slots, a.width = p->width, a.pages = p->pages, a.page = p->page_rows;
-        if (one_cta(*p)) launch(s, dim3(1), dim3(1024), shared_marks(k_pages_step, *p), k_pages_step, a);
-        else {
-            check(cudaMemsetAsync(a.keeper, 0, size_t(p->pages) * 4, s), "memset");
-            launch(s, table_grid(*p), dim3(256), 0, k_pages_gather, a);
-            launch(s, dim3(1), dim3(1024), 0, k_pages_assign, a);
-        }
-        copy_pages(*p, a.copies, a.copies + 3 * p->slots, s);
-    });
+    return guarded_op(err, err_len, [&] { step_pages(p, parents, counts, new_table, new_lengths, info, workspace, workspace_bytes, true, cudaStream_t(stream)); });
+}
+
+int chroma_b200_step_pages_uncut(const chroma_b200_pages* p, const int32_t* parents, const int32_t* counts, int32_t* new_table,
+                                 int32_t* new_lengths, int32_t* info, void* workspace, int64_t workspace_bytes, void* stream,
+                                 char* err, size_t err_len) {
+    return guarded_op(err, err_len, [&] { step_pages(p, parents, counts, new_table, new_lengths, info, workspace, workspace_bytes, false, cudaStream_t(stream)); });
 }
 
 int chroma_b200_compact_pages(const chroma_b200_pages* p, int32_t* new_table, int32_t* info, void* workspace,

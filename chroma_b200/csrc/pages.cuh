@@ -9,6 +9,8 @@
 // HBM: compaction of 64 sequences of 500-2,500 in four layers (1 GB moved) takes 172-180 us in all, 5.7 TB/s.
 #pragma once
 
+#include <limits.h>
+
 #include "paged.cuh"
 
 namespace cb200 {
@@ -22,6 +24,7 @@ struct StepArgs {
     int* free_list;     // [pages]
     int* copies;        // [slots][3]: source page, target page, rows; copies[3 * slots]: how many
     int slots, width, pages, page;
+    int cut;            // new lengths end where the table does
 };
 
 // One layer's pools and the layout of a page: `rows` rows of `heads` runs of `run` 16-byte words, the strides in
@@ -34,15 +37,17 @@ struct PoolArgs {
 
 __device__ __forceinline__ int pages_of(int rows, int page) { return rows / page + (rows % page != 0); }
 
-struct SlotStep { int parent, old_rows, new_rows; };
+// old_rows, new_rows: rows within what the table can name.
+struct SlotStep { int parent, old_rows, new_rows, new_length; };
 
 __device__ __forceinline__ SlotStep slot_step(const StepArgs& a, int slot) {
-    SlotStep s{a.parents[slot], 0, 0};
+    SlotStep s{a.parents[slot], 0, 0, 0};
     if (s.parent < 0 || s.parent >= a.slots) s.parent = -1;
     if (s.parent >= 0) {
         s.old_rows = held_rows(a.lengths, s.parent, a.width, a.page);
-        const int64_t want = int64_t(s.old_rows) + max(0, a.counts[slot]), most = int64_t(a.width) * a.page;
+        const int64_t more = max(0, a.counts[slot]), want = s.old_rows + more, most = int64_t(a.width) * a.page;
         s.new_rows = int(want < most ? want : most);
+        s.new_length = a.cut ? s.new_rows : int(min(length_of(a.lengths, s.parent) + more, int64_t(INT_MAX)));
     }
     return s;
 }
@@ -89,7 +94,7 @@ __device__ __forceinline__ void gather_entry(const StepArgs& a, const SlotStep& 
 [[maybe_unused]] static __global__ void __launch_bounds__(256) k_pages_gather(StepArgs a) {
     const int m = blockIdx.x * 256 + threadIdx.x;
     const SlotStep s = slot_step(a, blockIdx.y);
-    if (m == 0) a.new_lengths[blockIdx.y] = s.new_rows;
+    if (m == 0) a.new_lengths[blockIdx.y] = s.new_length;
     if (m < a.width) gather_entry(a, s, a.keeper, blockIdx.y, m);
 }
 
@@ -118,7 +123,7 @@ __device__ __forceinline__ void assign_pages(const StepArgs& a, const unsigned* 
     int taken = 0;
     for (int base = 0; base < a.slots; base += 1024) {
         const int slot = base + threadIdx.x;
-        SlotStep s{-1, 0, 0};
+        SlotStep s{-1, 0, 0, 0};
         int copy = 0, fresh = 0, held = 0, source = -1;
         int* row = a.new_table + int64_t(slot) * a.width;
         if (slot < a.slots) {
@@ -170,7 +175,7 @@ __device__ __forceinline__ void assign_pages(const StepArgs& a, const unsigned* 
     for (int slot = threadIdx.x; slot < a.slots; slot += 1024) {
         const SlotStep s = slot_step(a, slot);
         steps[slot] = s;
-        a.new_lengths[slot] = s.new_rows;
+        a.new_lengths[slot] = s.new_length;
     }
     for (int p = threadIdx.x; p < a.pages; p += 1024) page_marks[p] = 0;
     __syncthreads();

@@ -28,6 +28,7 @@ struct Entries {
     ENTRY(paged_attention);
     ENTRY(attention_workspace);
     ENTRY(step_pages);
+    ENTRY(step_pages_uncut);
     ENTRY(compact_pages);
     ENTRY(pages_workspace);
     ENTRY(process_logits);
@@ -47,6 +48,12 @@ int integer(PyObject* o, const char* name) {
     if (v == -1 && PyErr_Occurred()) throw python_error();
     TORCH_CHECK_VALUE(v >= 0 && v <= INT32_MAX, name, " must be nonnegative, got ", v);
     return int(v);
+}
+
+bool truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw python_error();
+    return v;
 }
 
 int storage_of(const Tensor& t, const char* what) {
@@ -198,7 +205,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 PyObject* step_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    count_args(n, 6);
+    count_args(n, 7);
     const Tensor &table = tensor(args[0], "table"), &lengths = tensor(args[1], "lengths"), &keys = tensor(args[4], "keys");
     const Call call(keys);
     const auto p = pages_of(call, keys, tensor(args[5], "values"), table, lengths, true);
@@ -207,7 +214,8 @@ PyObject* step_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor new_table = call.empty({p.slots, p.width}, at::kInt), new_lengths = call.empty({p.slots}, at::kInt), info = call.empty({3}, at::kInt),
                  workspace = call.empty({room}, at::kByte);
     char err[512];
-    run(native.step_pages(&p, parents, counts, new_table.data_ptr<int32_t>(), new_lengths.data_ptr<int32_t>(), info.data_ptr<int32_t>(),
+    const int cut = truth(args[6]);
+    run((cut ? native.step_pages : native.step_pages_uncut)(&p, parents, counts, new_table.data_ptr<int32_t>(), new_lengths.data_ptr<int32_t>(), info.data_ptr<int32_t>(),
                           workspace.data_ptr(), room, call.stream(), err, sizeof err), err);
     return Py_BuildValue("(NNN)", THPVariable_Wrap(new_table), THPVariable_Wrap(new_lengths), THPVariable_Wrap(info));
     END_HANDLE_TH_ERRORS
@@ -312,9 +320,10 @@ PyObject* process_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // bind(addresses): the entry points of the native library, in the order of Entries.
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    void* at[8];
-    count_args(n, 8);
-    for (int i = 0; i < 8; ++i) {
+    constexpr int kEntries = sizeof(Entries) / sizeof(void*);
+    void* at[kEntries];
+    count_args(n, kEntries);
+    for (int i = 0; i < kEntries; ++i) {
         at[i] = PyLong_AsVoidPtr(args[i]);
         if (PyErr_Occurred()) throw python_error();
     }
@@ -324,6 +333,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     ENTRY(paged_attention);
     ENTRY(attention_workspace);
     ENTRY(step_pages);
+    ENTRY(step_pages_uncut);
     ENTRY(compact_pages);
     ENTRY(pages_workspace);
     ENTRY(process_logits);

@@ -37,7 +37,7 @@ class PagedModel:
     def reserve(self, parents: Tensor, counts: Tensor) -> Tensor:
         """Slot s goes on from slot ``parents[s]`` with ``counts[s]`` new rows; returns [pages free, short, copied]."""
         self.table, self.lengths, info = chroma_b200.step_pages(self.table, self.lengths, parents, counts, self.keys,
-                                                                self.values)
+                                                                self.values, cut=False)
         return info
 
     def compact(self) -> Tensor:

@@ -293,11 +293,17 @@ int64_t chroma_b200_attention_workspace(const chroma_b200_pages* pages, const ch
  * pages short, pages copied}. A page that no slot holds is free. Free pages are given out from the lowest number, to
  * slots from the lowest. A slot that will write into a page which another slot holds too gets a copy of its rows (all
  * layers) first; the holder with the most rows in that page, the lowest slot among equals, keeps it. With too few
- * free pages the last entries stay -1; a length that passes width * page_rows is cut there. Neither output may be an
- * input. `workspace`: chroma_b200_pages_workspace bytes. */
+ * free pages the last entries stay -1; a length that passes width * page_rows is cut there, and the rows that were asked
+ * for past it must not be appended (they would be taken for the rows before the end). Neither output may be an input.
+ * `workspace`: chroma_b200_pages_workspace bytes. */
 int chroma_b200_step_pages(const chroma_b200_pages* pages, const int32_t* parents, const int32_t* counts,
                            int32_t* new_table, int32_t* new_lengths, int32_t* info, void* workspace,
                            int64_t workspace_bytes, void* stream, char* err, size_t err_len);
+/* The same, but lengths go on past the table's end: appended rows whose positions lie there are dropped, and a length above
+ * width * page_rows tells that the sequence has outgrown its table. */
+int chroma_b200_step_pages_uncut(const chroma_b200_pages* pages, const int32_t* parents, const int32_t* counts,
+                                 int32_t* new_table, int32_t* new_lengths, int32_t* info, void* workspace,
+                                 int64_t workspace_bytes, void* stream, char* err, size_t err_len);
 /* Moves the n pages that slots hold to numbers below n: the i-th held page from n up goes to the i-th free page
  * below n, all layers. Writes the new table [slots][width] (not the input's memory) and info[2] = {n, moved}. */
 int chroma_b200_compact_pages(const chroma_b200_pages* pages, int32_t* new_table, int32_t* info, void* workspace,

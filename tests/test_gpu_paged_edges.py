@@ -146,3 +146,33 @@ def test_long_caches_past_the_table(gpu) -> None:  # type: ignore[no-untyped-def
                 want = ref.attention(q, k, v, wide, n, starts, scale=0.2, window=window, first=window // 300)
                 got, logs = chroma_b200.paged_attention(q, k, v, table, n, starts, scale=0.2, window=window, first=window // 300, lse=True)
                 check(got, want, dtype=dtype, dim=dim, lse=logs)
+
+
+@pytest.mark.parametrize("slots,width,page", [(4, 3, 4), (70, 1000, 2)])  # decided by one CTA, and by several launches
+def test_steps_past_the_table_write_over_nothing(gpu, slots, width, page) -> None:  # type: ignore[no-untyped-def]
+    end = width * page
+    lengths = [end, end - 1, 0, 2] + [0] * (slots - 4)
+    k, v, table, n = cache(lengths, dtype=F32, kv=1, dim=16, page=page, width=width, spare=9, poison=False)
+    ints = lambda x: torch.tensor(x + [-1] * (slots - len(x)), dtype=torch.int32).cuda()  # noqa: E731
+    # A full sequence is forked, one that is full but for a row goes on by three.
+    parents, counts = ints([0, 1, 0, 3]), ints([1, 3, 2, 1])
+    want, _, info, copies = ref.step(table.cpu().numpy(), n.cpu().numpy(), parents.tolist(), counts.tolist(), len(k), page)
+    before = k.clone()
+    new, length, got = chroma_b200.step_pages(table, n, parents, counts, k[None], v[None], cut=False)
+    assert new.tolist() == want.tolist() and got.tolist() == info
+    assert length.tolist() == [end + 1, end + 2, end + 2, 3] + [0] * (slots - 4)
+    for a, b, rows in copies:
+        before[b, :rows] = before[a, :rows]
+    starts = torch.tensor([0, 1, 4, 6] + [7] * (slots - 3), dtype=torch.int32).cuda()
+    rows = torch.randn(7, 1, 16, device="cuda")
+    chroma_b200.paged_append(k, v, rows, rows, new, length, starts)
+    before[new[1, width - 1], page - 1] = rows[1]
+    before[new[3, 2 // page], 2 % page] = rows[6]
+    assert torch.equal(k, before)
+    # once more, from there; a length stays below 2^31
+    new, length, got = chroma_b200.step_pages(new, length, ints([0, 0, 2, 3]), ints([5, 2**31 - 1, 0, 0]), k[None], v[None], cut=False)
+    assert length.tolist() == [end + 6, 2**31 - 1, end + 2, 3] + [0] * (slots - 4) and got.tolist()[1:] == [0, 0]
+    assert torch.equal(k, before)
+    # cut at the end, as without the argument
+    for more in ({}, {"cut": True}):
+        assert chroma_b200.step_pages(new, length, ints([0, 1, 2, 3]), ints([5, 0, 0, 1]), k[None], v[None], **more)[1].tolist()[:4] == [end, end, end, 4]
