@@ -31,7 +31,7 @@
 // A position that no row may see costs nothing (whole tiles are passed over) or a mask of 128 bits per row, applied only
 // to the tiles that need it. Values behind the end of a sequence are cleared in shared memory, since what lies there may
 // not be finite. Positions that some rows of a tile see and others do not meet the others with weight 0, which is no
-// protection against infinities: a row whose result is not finite is computed again, key by key.
+// protection against infinities: a CTA that finds one in a result takes its items a second time, with such values cleaned.
 //
 // Where there are few items (a short chunk after a long cache), the keys of each are split over several CTAs, which leave
 // fp32 partial results for k_prompt_join (16 tokens after 16,000, 64/8 heads of 64: 69 us, without splits 203).
@@ -39,9 +39,9 @@
 // All waits are bounded (tma.cuh).
 #pragma once
 
-#include "mma.cuh"
-#include "paged.cuh"
-#include "tcgen05.cuh"
+#include <type_traits>
+
+#include "paged_decode.cuh"
 
 namespace cb200 {
 
@@ -125,6 +125,7 @@ struct PromptItem {
     int tiles, skip, pre, main0;              // key tiles of the split, after `skip`: of [0, pre), then from main0 on
     int active;                               // tiles of rows: 1 or 2
     int64_t part;                             // number of this split's first row
+    unsigned number;                          // of all splits of all items
     __device__ __forceinline__ int key0(int t) const { return (skip + t < pre ? skip + t : main0 + skip + t - pre) * kPrTile; }
 };
 
@@ -137,8 +138,23 @@ __device__ __forceinline__ uint32_t* prompt_order() {
 struct PromptCursor {
     int slot, before, round;  // tiles of the slots after `slot`
     bool sorted;              // or prompt_order() has slot << 16 | tile of each place
+    bool second = false;      // the second time
     __device__ __forceinline__ explicit PromptCursor(const PagedArgs& a, bool in_order = false)
         : slot(a.slots - 1), before(0), round(0), sorted(in_order) {}
+    // The end of the first time, for every warp of the CTA.
+    static __device__ __forceinline__ void end_first() {
+        __syncwarp();
+        asm volatile("bar.sync 1, %0;" ::"n"(kPrThreads) : "memory");
+    }
+    // After the last item: back to the first if `bad` says so by then.
+    __device__ __forceinline__ bool again(const PagedPromptArgs& p, const volatile int& bad) {
+        if (second) return false;
+        second = true;
+        end_first();
+        slot = p.a.slots - 1;
+        before = round = 0;
+        return bad;
+    }
     static __device__ __forceinline__ int rows_of(const PagedArgs& a, int s) {
         const int t0 = min(max(a.starts[s], 0), a.tokens), t1 = min(max(a.starts[s + 1], 0), a.tokens);
         return max(0, t1 - t0) * a.group;
@@ -154,6 +170,11 @@ struct PromptCursor {
         const unsigned i = unsigned(round) * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         ++round;
         if (i >= unsigned(total) * unsigned(p.a.kv) * unsigned(p.splits)) return false;
+        take(p, i, w);
+        return true;
+    }
+    // Number i of all splits of all items.
+    __device__ __forceinline__ void take(const PagedPromptArgs& p, unsigned i, PromptItem& w) {
         find(p, p.splits == 1 ? i : p.by_splits.div(i), w);
         if (p.splits > 1) {
             const int z = int(i - p.by_splits.div(i) * unsigned(p.splits)), all = w.tiles;
@@ -161,7 +182,7 @@ struct PromptCursor {
             w.tiles = int(int64_t(all) * (z + 1) / p.splits) - w.skip;
             w.part = int64_t(i) * 256;
         }
-        return true;
+        w.number = i;
     }
     // Item i of all (a later one than the last).
     __device__ __forceinline__ void find(const PagedPromptArgs& p, unsigned i, PromptItem& w) {
@@ -200,67 +221,87 @@ struct PromptCursor {
     }
 };
 
-// Softmax attention of one row, key by key, by one warp: any mask, any values. o[c] is dim 32 c + lane.
-template <typename T>
-__device__ __noinline__ void attend_row(const PagedArgs& a, int token, int head, int slot, int pos, float& m, float& l,
-                                        float (&o)[4]) {
-    const int lane = threadIdx.x & 31, kvh = head / a.group;
-    const T* q = static_cast<const T*>(a.q) + token * a.qt + head * a.qh;
-    m = -INFINITY;
-    l = 0.f;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] = 0.f;
-    const int low = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    const int top = min(pos, a.width * a.page - 1);
-    const int first = min(a.first, min(low, top + 1));  // [0, first) then [low, top]
-    const int total = first + max(0, top + 1 - low);
-    for (int base = 0; base < total; base += 32) {
-        const int i = base + lane;
-        const int j = i < first ? i : low + i - first;
-        const int entry = i < total ? int(a.by_page.div(uint32_t(j))) : 0;
-        int id = i < total ? a.table[slot * a.ts + entry] : -1;
-        if (id >= a.pages) id = -1;
-        float s = -INFINITY;
-        const int row = j - entry * a.page;
-        if (id >= 0) {
-            const T* k = static_cast<const T*>(a.k) + id * a.kp + row * a.kr + kvh * a.kh;
-            float dot = 0.f;
-            for (int d = 0; d < a.dim; ++d) dot = fmaf(Store<T>::load(q + d), Store<T>::load(k + d), dot);
-            s = dot * a.scale_log2;
-        }
-        const float mx = fmaxf(m, warp_max(s));
-        if (mx == -INFINITY && !__any_sync(0xffffffffu, isnan(s))) continue;
-        const float corr = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - mx);
-        const float p = id < 0 ? 0.f : exp2f(s - mx);
-        l = l * corr + warp_sum(p);
-        m = mx;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] *= corr;
-        for (int e = 0; e < min(32, total - base); ++e) {
-            const int ide = __shfl_sync(0xffffffffu, id, e), rowe = __shfl_sync(0xffffffffu, row, e);
-            const float pe = __shfl_sync(0xffffffffu, p, e);
-            if (ide < 0) continue;
-            const T* v = static_cast<const T*>(a.v) + ide * a.vp + rowe * a.vr + kvh * a.vh;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (c * 32 + lane < a.dim) o[c] = fmaf(pe, Store<T>::load(v + c * 32 + lane), o[c]);
-        }
-    }
+// ---- Values that are not finite. A weight of 0 does not keep them from a row that does not see them. So where a row's result is
+// not finite although its sum of weights is (a score that is not finite makes the sum so, and belongs to a key that the row sees,
+// since others are replaced), the CTA takes its items a second time. Then the values of tiles of keys that not every row of a
+// tile sees are cleaned in shared memory, and each row is given what it sees of them afterwards. The second time costs as much
+// as the first, and a pass over the values of those tiles: 600 tokens after 6,000, 16/8 heads of 64, 0.1 ms and 0.7 with one bad
+// value among them; computing such rows again one by one, while the pipeline waited, took 112.
+//
+// Everything for the second time is inlined and takes its arguments anew from the item's number: calls from the loop over the
+// items, though never made, cost the first time 2 to 4% (four prompts of 2,048: 293 us for 283).
+
+// Whether every row of tile k of an item sees every position of the tile of keys at j0.
+__device__ __forceinline__ bool whole_tile(const PagedPromptArgs& p, const PromptItem& w, int k, int j0) {
+    const int first = w.pos0 + int(p.by_group.div(w.row0 + k * kPrTile));
+    const int last = w.pos0 + int(p.by_group.div(min(w.row0 + (k + 1) * kPrTile, w.rows) - 1));
+    return j0 + kPrTile - 1 <= first && (p.a.window <= 0 || last - j0 < p.a.window || j0 + kPrTile <= p.a.first);
 }
 
-// Writes what attend_row found.
-template <typename T>
-__device__ __forceinline__ void finish_row(const PagedArgs& a, int token, int head, float m, float l, const float (&o)[4]) {
-    const int lane = threadIdx.x & 31;
-    const float sink = sink_log2<T>(a.sinks, a.sinks_fp32, head);
-    const float top = fmaxf(m, sink);
-    const float c = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - top);
-    const float sum = l * c + (sink == -INFINITY ? 0.f : exp2f(sink - top));
-    T* orow = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (e * 32 + lane < a.dim) Store<T>::store(orow + e * 32 + lane, sum == 0.f ? 0.f : o[e] * c / sum);
-    if (a.lse && lane == 0) a.lse[int64_t(token) * a.heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+__device__ __forceinline__ bool has_bad(const uint4& x) {
+    const auto bad = [](uint32_t v) { return (v & 0x7f80) == 0x7f80 || (v & 0x7f800000) == 0x7f800000; };
+    return bad(x.x) || bad(x.y) || bad(x.z) || bad(x.w);
+}
+__device__ __forceinline__ uint32_t cleaned(uint32_t x) {
+    return ((x & 0x7f80) == 0x7f80 ? 0u : x & 0xffffu) | ((x & 0x7f800000) == 0x7f800000 ? 0u : x & 0xffff0000u);
+}
+
+// Row r of a tile of values in shared memory without what is not finite; true if there was something.
+template <int H> __device__ __forceinline__ bool clean_row(uint8_t* tile, int r) {
+    bool found = false;
+    for (int c = 0; c < 8 * H; ++c) {
+        uint4* at = reinterpret_cast<uint4*>(tile + (c >> 3) * PromptShape<H>::kBlock + r * 128 + (((c ^ r) & 7) << 4));
+        uint4 x = *at;
+        if (!has_bad(x)) continue;
+        found = true;
+        *at = make_uint4(cleaned(x.x), cleaned(x.y), cleaned(x.z), cleaned(x.w));
+    }
+    return found;
+}
+
+// A softmax thread's row of item `number`.
+template <int H> struct SecondLook {
+    PromptItem w;
+    int pos = -1;
+    __nv_bfloat16* out = nullptr;  // the row's result, or its part of a split's
+    float* part = nullptr;
+    __device__ __forceinline__ SecondLook(const PagedPromptArgs& p, unsigned number, bool sorted) {
+        PromptCursor(p.a, sorted).take(p, number, w);
+        const int row = w.row0 + threadIdx.x, n = int(p.by_group.div(row));
+        if (row >= w.rows) return;
+        pos = w.pos0 + n;
+        out = static_cast<__nv_bfloat16*>(p.a.out) + (w.token0 + n) * p.a.ot + (w.kvh * p.a.group + row - n * p.a.group) * p.a.oh;
+        part = p.splits > 1 ? p.parts + (w.part + threadIdx.x) * (64 * H) : nullptr;
+    }
+};
+
+// Adds to a thread's row what it sees of the values that were cleaned.
+template <int H> __device__ __forceinline__ void add_cleaned(const PagedPromptArgs& p, unsigned number, bool sorted) {
+    const PagedArgs& a = p.a;
+    const SecondLook<H> look(p, number, sorted);
+    const PromptItem& w = look.w;
+#pragma unroll 1
+    for (int t = 0; t < w.tiles; ++t) {
+        const int t0 = w.key0(t);
+        if (whole_tile(p, w, 0, t0) && (w.active == 1 || whole_tile(p, w, 1, t0))) continue;
+#pragma unroll 1
+        for (int j = t0; j < t0 + kPrTile; ++j) {
+            const int entry = int(a.by_page.div(uint32_t(j))), id = entry < a.width ? __ldg(a.table + w.slot * a.ts + entry) : -1;
+            if (id < 0 || id >= a.pages) continue;
+            const auto* v = static_cast<const __nv_bfloat16*>(a.v) + id * a.vp + (j - entry * a.page) * a.vr + w.kvh * a.vh;
+#pragma unroll 1
+            for (int d = 0; d < a.dim; d += 8) {
+                if (!has_bad(__ldg(reinterpret_cast<const uint4*>(v + d))) || look.pos < 0 || !sees(look.pos, j, a.window, a.first)) continue;
+#pragma unroll 1
+                for (int e = d; e < d + 8; ++e) {
+                    const float x = __bfloat162float(v[e]);
+                    if (x * 0.f == 0.f) continue;
+                    if (look.part) look.part[e] += x;
+                    else look.out[e] = __float2bfloat16_rn(__bfloat162float(look.out[e]) + x);
+                }
+            }
+        }
+    }
 }
 
 __device__ __forceinline__ uint32_t bits_from_to(int lo, int hi) {  // bits lo..hi of a word, cut to it
@@ -287,7 +328,7 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
     __shared__ uint32_t tmem_base;
     __shared__ int tile_counts[kPrSortedSlots];
     __shared__ unsigned long long s_total;
-    __shared__ volatile int abort_flag;
+    __shared__ volatile int abort_flag, bad_flag, cleaned_flag;  // bad_flag: a result is not finite; cleaned_flag: a value was cleaned
     const PagedArgs& a = p.a;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
@@ -304,7 +345,7 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
             mbar_init(&kv_full[s], 1);
             mbar_init(&kv_empty[s], 1);
         }
-        abort_flag = 0;
+        abort_flag = bad_flag = cleaned_flag = 0;
         s_total = 0;
         fence_barrier_init();
     }
@@ -333,15 +374,19 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
         }
         __syncthreads();
     }
-    PromptCursor cursor(a, sorted);
-    PromptItem w;
 
     if (warp >= 8) {
+    PromptCursor cursor(a, sorted);
+    PromptItem w;
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrOtherRegs));
     if (warp == 9) {
         // ---- K and V
         int g = 0;  // tiles so far
-        while (!abort_flag && cursor.next(p, total, w)) {
+        while (!abort_flag) {
+            if (!cursor.next(p, total, w)) {
+                if (cursor.again(p, bad_flag)) continue;
+                break;
+            }
             for (int t = 0; t < w.tiles; ++t, ++g) {
                 const int s = g % kStages;
                 if (!mbar_wait(&kv_empty[s], unsigned((g / kStages) & 1) ^ 1, p.error)) abort_flag = 1;
@@ -410,6 +455,7 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
                 }
             }
         }
+        if (!cursor.second) cursor.end_first();
         if (abort_flag)  // after a wait that gave up: the copies under way end (or are given up) before the memory is left
             for (int i = max(0, g - kStages); i < g; ++i)
                 if (!mbar_wait(&kv_full[i % kStages], unsigned((i / kStages) & 1), p.error)) break;
@@ -417,7 +463,11 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
         // ---- Q of tile `warp - 10`
         const int k = warp - 10;
         int loads = 0;
-        while (!abort_flag && cursor.next(p, total, w)) {
+        while (!abort_flag) {
+            if (!cursor.next(p, total, w)) {
+                if (cursor.again(p, bad_flag)) continue;
+                break;
+            }
             if (!w.tiles || k >= w.active) continue;
             if (!mbar_wait(&q_empty[k], unsigned(loads & 1) ^ 1, p.error)) abort_flag = 1;
             if (abort_flag) break;
@@ -451,6 +501,7 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[k]);
         }
+        if (!cursor.second) cursor.end_first();
         if (abort_flag && loads) mbar_wait(&q_full[k], unsigned(loads - 1) & 1, p.error);
     } else if (warp == 8) {
         // ---- products, ping-pong over the two tiles of rows; the warp stays converged
@@ -485,7 +536,11 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
             if (k == w.active - 1) umma_commit_elected(&kv_empty[tile % kStages]);
             return true;
         };
-        while (!abort_flag && cursor.next(p, total, w)) {
+        while (!abort_flag) {
+            if (!cursor.next(p, total, w)) {
+                if (cursor.again(p, bad_flag)) continue;
+                break;
+            }
             if (!w.tiles) continue;
             const bool two = w.active == 2;
             bool ok = wait(&kv_full[g % kStages], g / kStages);
@@ -509,6 +564,7 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
                 if (abort_flag) ok = false;
             }
         }
+        if (!cursor.second) cursor.end_first();
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPrSoftmaxRegs));
@@ -518,7 +574,13 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
         const uint32_t tS = tmem + uint32_t(k * kPrTile) + lanes, tO = tmem + uint32_t(kO + k * D) + lanes;
         const uint32_t tP = kOwnP ? tmem + uint32_t(2 * kPrTile + k * 64) + lanes : tS;
         int g = 0, uses = 0, ends = 0;
-        while (!abort_flag && cursor.next(p, total, w)) {
+        PromptCursor cursor(a, sorted);
+        PromptItem w;
+        while (!abort_flag) {
+            if (!cursor.next(p, total, w)) {
+                if (cursor.again(p, bad_flag)) continue;
+                break;
+            }
             if (k >= w.active) {
                 g += w.tiles;
                 continue;
@@ -538,8 +600,12 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
                 const int s = g % kStages, j0 = w.key0(t);
                 if (!mbar_wait(&kv_full[s], unsigned((g / kStages) & 1), p.error)) abort_flag = 1;
                 const uint4 none = *reinterpret_cast<const uint4*>(gone + s * 4);
-                const bool all = j0 + kPrTile - 1 <= pos_first && (a.window <= 0 || pos_last - j0 < a.window || j0 + kPrTile <= a.first) &&
-                                 !(none.x | none.y | none.z | none.w);
+                const bool whole = j0 + kPrTile - 1 <= pos_first && (a.window <= 0 || pos_last - j0 < a.window || j0 + kPrTile <= a.first);
+                const bool all = whole && !(none.x | none.y | none.z | none.w);
+                if (cursor.second && !whole) {
+                    if (clean_row<H>(KV + s * Shape::kStage + Shape::kTile, r)) cleaned_flag = 1;
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
                 if (!mbar_wait(&s_full[k], unsigned(uses++ & 1), p.error)) abort_flag = 1;
                 if (abort_flag) break;
                 tc_fence_after();
@@ -625,6 +691,7 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
             }
             if (abort_flag) break;
             // ---- the item's end
+            float check = 0.f;  // NaN as soon as something is not finite
             if (p.splits > 1) {
                 const int64_t at = w.part + k * kPrTile + r;
                 if (w.tiles) {
@@ -636,14 +703,17 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
                         float ov[32];
                         tmem_load32(tO + c * 32, ov);
 #pragma unroll
+                        for (int e = 0; e < 32; ++e) check = fmaf(ov[e], 0.f, check);
+#pragma unroll
                         for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(p.parts + at * D + c * 32 + e) = make_float4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
                     }
+                    if (row_ok && check != 0.f && l_run * 0.f == 0.f) bad_flag = 1;
+                    if (cursor.second && cleaned_flag) add_cleaned<H>(p, w.number, sorted);
                 }
                 p.part_ml[at] = make_float2(m_run, l_run);
                 tc_fence_before();
                 continue;
             }
-            bool again = false;
             const float top = fmaxf(m_run, sink);
             const float c0 = m_run == -INFINITY ? (l_run == 0.f ? 0.f : 1.f) : fast_exp2(m_run - top);
             const float sum = l_run * c0 + (sink == -INFINITY ? 0.f : fast_exp2(sink - top));
@@ -653,7 +723,6 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
                 if (!mbar_wait(&o_done[k], unsigned((kOwnP ? uses - 1 : ends++) & 1), p.error)) abort_flag = 1;
                 if (abort_flag) break;
                 tc_fence_after();
-                float check = l_run * 0.f;  // NaN as soon as something is not finite
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
                     float ov[32];
@@ -674,21 +743,15 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
                                 for (int u = 0; u < 8; ++u) reinterpret_cast<uint16_t*>(orow + d)[u] = uint16_t(w4[u >> 1] >> (16 * (u & 1)));
                         }
                 }
-                again = row_ok && check != 0.f;
+                if (row_ok && check != 0.f && l_run * 0.f == 0.f) bad_flag = 1;
+                if (cursor.second && cleaned_flag) add_cleaned<H>(p, w.number, sorted);
             } else if (row_ok) {
                 for (int d = 0; d < a.dim; ++d) orow[d] = __float2bfloat16_rn(0.f);
             }
             if (a.lse && row_ok) a.lse[int64_t(token) * a.heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
-            for (uint32_t bad = __ballot_sync(0xffffffffu, again); bad; bad &= bad - 1) {
-                const int from = __ffs(bad) - 1;
-                const int tk = __shfl_sync(0xffffffffu, token, from), hd = __shfl_sync(0xffffffffu, head, from), ps = __shfl_sync(0xffffffffu, pos, from);
-                float m, l, o[4];
-                attend_row<__nv_bfloat16>(a, tk, hd, w.slot, ps, m, l, o);
-                __syncwarp();
-                finish_row<__nv_bfloat16>(a, tk, hd, m, l, o);
-            }
             tc_fence_before();  // O has been read before its next products are asked for
         }
+        if (!cursor.second) cursor.end_first();
     }
     tc_fence_before();
     __syncthreads();
@@ -698,8 +761,7 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
     }
 }
 
-// Joins the splits of every row, in their order: a warp per row, 32 rows of an item a CTA. A row whose sum is not finite is
-// computed again.
+// Joins the splits of every row, in their order: a warp per row, 32 rows of an item a CTA.
 template <int H> __global__ void __launch_bounds__(256) k_prompt_join(const __grid_constant__ PagedPromptArgs p) {
     constexpr int D = 64 * H;
     __shared__ unsigned long long s_total;
@@ -731,15 +793,12 @@ template <int H> __global__ void __launch_bounds__(256) k_prompt_join(const __gr
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) x[c] += p.parts[part(z) * D + c * 32 + lane] * weight;
         }
-        float check = sum * 0.f;
+        const HeadEnd end = head_end(top, sum, sink_log2<__nv_bfloat16>(a.sinks, a.sinks_fp32, head));
+        __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(a.out) + token * a.ot + head * a.oh;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) check = fmaf(x[c], 0.f, check);
-        float o[4];
-        if (__any_sync(0xffffffffu, check != 0.f)) attend_row<__nv_bfloat16>(a, token, head, w.slot, w.pos0 + number, top, sum, o);
-        else
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[c] = c < D / 32 ? x[c] : 0.f;
-        finish_row<__nv_bfloat16>(a, token, head, top, sum, o);
+        for (int c = 0; c < D / 32; ++c)
+            if (c * 32 + lane < a.dim) orow[c * 32 + lane] = __float2bfloat16_rn(end.inv == 0.f ? 0.f : x[c] * end.c * end.inv);
+        if (a.lse && lane == 0) a.lse[int64_t(token) * a.heads + head] = end.lse;
     }
 }
 

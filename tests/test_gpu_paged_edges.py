@@ -176,3 +176,78 @@ def test_steps_past_the_table_write_over_nothing(gpu, slots, width, page) -> Non
     # cut at the end, as without the argument
     for more in ({}, {"cut": True}):
         assert chroma_b200.step_pages(new, length, ints([0, 1, 2, 3]), ints([5, 0, 0, 1]), k[None], v[None], **more)[1].tolist()[:4] == [end, end, end, 4]
+
+
+# ---- values that are not finite
+
+def agree(got, want, *, dtype, dim, scale_of):  # type: ignore[no-untyped-def]
+    """Entries are finite where the 64-bit form's are, and then near them; ``scale_of``: the same without the bad values."""
+    got, out = got.double().cpu(), want[0]
+    fine = torch.isfinite(out)
+    assert torch.equal(torch.isfinite(got), fine)
+    a, r, _ = ref.attention_tolerance(dtype, dim, scale_of[2], scale_of[3])
+    assert bool(((got - out)[fine].abs() <= a + r * out[fine].abs()).all())
+
+
+BAD = [("k", 40, slice(None), float("nan")), ("v", 40, slice(None), float("nan")), ("v", 101, 3, float("inf")),
+       ("v", 101, 9, float("nan")), ("v", 33, 3, float("-inf")), ("k", 130, slice(2, 5), float("inf")), ("v", 0, 1, float("nan"))]
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,page", [(F32, 4, 2, 16, 16), (B16, 8, 2, 64, 16), (B16, 4, 1, 128, 24), (B16, 3, 1, 80, 5)])
+@pytest.mark.parametrize("window,first", [(0, 0), (30, 0), (25, 2)])
+@pytest.mark.parametrize("bad", [BAD[:1], BAD[1:2], BAD[2:3], BAD[2:5], BAD[5:], BAD], ids=range(6))
+def test_rows_that_see_values_that_are_not_finite(gpu, dtype, heads, kv, dim, page, window, first, bad) -> None:  # type: ignore[no-untyped-def]
+    new, prior = 150, 20
+    k, v, table, n = cache([new + prior], dtype=dtype, kv=kv, dim=dim, page=page)
+    starts = torch.tensor([0, new], dtype=torch.int32).cuda()
+    q = queries(new, heads, dim, dtype)
+    clean = ref.attention(q, k, v, table, n, starts, scale=0.2, window=window, first=first)
+    for pool, p, d, x in bad:
+        (k if pool == "k" else v)[table[0, p // page].item(), p % page, 0, d] = x
+    want = ref.attention(q, k, v, table, n, starts, scale=0.2, window=window, first=first)
+    got = chroma_b200.paged_attention(q, k, v, table, n, starts, scale=0.2, window=window, first=first)
+    agree(got, want, dtype=dtype, dim=dim, scale_of=clean)
+    for length in (35, 41, 103, 170):  # single tokens
+        n[0] = length
+        want = ref.attention(q[:1], k, v, table, n, scale=0.2, window=window, first=first)
+        agree(chroma_b200.paged_attention(q[:1], k, v, table, n, scale=0.2, window=window, first=first), want, dtype=dtype, dim=dim, scale_of=clean)
+
+
+@pytest.mark.parametrize("what", ["key", "value", "one entry", "late value"])
+@pytest.mark.parametrize("heads,kv,dim,new", [(16, 8, 64, 600), (16, 8, 128, 600), (16, 2, 64, 20)])  # the last: keys are split
+def test_bad_values_in_a_long_cache(gpu, what, heads, kv, dim, new) -> None:  # type: ignore[no-untyped-def]
+    """Rows that see them are not finite, the others are as without them, and the call takes about as long."""
+    prior, page, dtype = 6000, 16, B16
+    k, v, table, n = cache([prior + new, new + 5], dtype=dtype, kv=kv, dim=dim, page=page)
+    starts = torch.tensor([0, new, 2 * new], dtype=torch.int32).cuda()
+    q = queries(2 * new, heads, dim, dtype)
+
+    def timed():  # type: ignore[no-untyped-def]
+        times = []
+        for _ in range(3):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            out = chroma_b200.paged_attention(q, k, v, table, n, starts)
+            end.record()
+            end.synchronize()
+            times.append(begin.elapsed_time(end))
+        return out, min(times)
+
+    clean, usual = timed()
+    p = 5 if what != "late value" else prior + new // 2
+    entries = slice(None) if what in ("key", "value") else 7
+    (k if what == "key" else v)[table[0, p // page], p % page, :, entries] = float("nan")
+    got, longer = timed()
+    chroma_b200.check_operators()
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[max(0, p - prior) : new, :, entries] = True
+    assert torch.equal(torch.isnan(got), hit)
+    # rows that shared a tile with a bad value but do not see it were computed another way
+    away = torch.ones_like(hit)
+    if what == "late value":
+        away[:new] = False
+        near = ~hit[:new]
+        assert float((got[:new] - clean[:new])[near].float().abs().max()) <= 2.0**-7 * float(clean.float().abs().max())
+    assert torch.equal(got[away & ~hit], clean[away & ~hit])
+    # 20 times and 5 ms: what is looked at again costs a pass over the values, not one over the cache for every row
+    assert longer <= 20 * usual + 5
