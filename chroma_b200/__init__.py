@@ -5,7 +5,8 @@ Public surface, as in the reference (chroma/__init__.py:14-26): ``compile``, ``P
 imports Torch on first use.
 
 Operators for serving over a paged key-value cache, on CUDA tensors: ``paged_append``, ``paged_attention``,
-``step_pages``, ``compact_pages``, and ``process_logits`` for the logits that follow.
+``step_pages``, ``compact_pages``, and ``process_logits`` for the logits that follow; ``check_operators``. They import Torch
+when they are first named, so ``from chroma_b200 import *`` leaves them out.
 """
 
 from __future__ import annotations
@@ -36,7 +37,7 @@ def compile_model(model: Any, output: str | Path, *, steps: int, context: int | 
 
 
 # Operators on CUDA tensors of the caller (a paged key-value cache, its attention, logits): Torch is imported by the
-# caller, who has the tensors.
+# caller, who has the tensors. Not in __all__, which a star import names one by one.
 _OPERATORS = {"paged_append": "paged", "paged_attention": "paged", "step_pages": "paged", "compact_pages": "paged",
               "check_operators": "paged", "process_logits": "logits"}
 
@@ -51,4 +52,8 @@ def __getattr__(name: str) -> Any:
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
-__all__ = ["BatchDecoder", "Decoder", "ExpertGroup", "Program", "compile", "compile_model", *_OPERATORS]
+__all__ = ["BatchDecoder", "Decoder", "ExpertGroup", "Program", "compile", "compile_model"]
+
+
+def __dir__() -> list[str]:
+    return sorted({*globals(), *_OPERATORS})
