@@ -22,6 +22,7 @@ nothing waits for the device or reads it from the host (``check_operators`` does
 from __future__ import annotations
 
 import ctypes
+import sysconfig
 from typing import Any
 
 import torch
@@ -37,8 +38,12 @@ def _module() -> Any:
     """The binding of the operators (chroma_b200/csrc/tensors.cpp), given the entry points of the native library."""
     assert torch.version.cuda, "the operators need a Torch that was built with CUDA"
     lib = nat.lib()
+    tag = f"torch {torch.__version__}, {sysconfig.get_config_var('SOABI')}"
     try:
         from chroma_b200._src import _tensors
+
+        if _tensors.built_for != tag:
+            raise ImportError(f"it is built for {_tensors.built_for}, this is {tag}")
     except ImportError as error:
         raise RuntimeError(f"the operators' binding is not built for this Torch ({error}); build it with "
                            "`python -m chroma_b200.build --force`") from error

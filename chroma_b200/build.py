@@ -2,12 +2,15 @@
 binding of the operators on CUDA tensors into ``chroma_b200/_src/_tensors.so``.
 
 nvcc cross-compiles without a GPU. The library links the CUDA runtime statically so it loads wherever the driver
-is present. The binding is built against the installed Torch; nothing but those operators needs it.
+is present. The binding is built against the installed Torch, and left out where there is none with CUDA; nothing but those
+operators needs it.
 """
 
 from __future__ import annotations
 
+import importlib.util
 import os
+import runpy
 import shutil
 import subprocess
 import sys
@@ -42,9 +45,21 @@ def tensors_command(target: Path = TENSORS) -> list[str]:
     home = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parents[1]
     return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", str(TENSORS_SOURCE), "-o", str(target),
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f'-DBUILT_FOR="{built_for()}"',
+            str(TENSORS_SOURCE), "-o", str(target),
             "-I", sysconfig.get_paths()["include"], "-isystem", str(home / "include"), "-isystem",
             str(cuda / "include"), "-L", str(home / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+
+
+def built_for() -> str | None:
+    """The Torch and the Python that a binding built now is for; None without a Torch that has CUDA. Torch is not imported."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        return None
+    version = runpy.run_path(str(Path(spec.submodule_search_locations[0]) / "version.py"))
+    if not version.get("cuda"):
+        return None
+    return f"torch {version['__version__']}, {sysconfig.get_config_var('SOABI')}"
 
 
 def stale(target: Path = TARGET, depends: list[Path] = DEPENDS) -> bool:
@@ -55,19 +70,33 @@ def stale(target: Path = TARGET, depends: list[Path] = DEPENDS) -> bool:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    jobs = []
-    for target, depends, make in ((TARGET, DEPENDS, command), (TENSORS, [TENSORS_SOURCE, *DEPENDS[-1:]], tensors_command)):
-        if force or stale(target, depends):
-            tmp = target.with_suffix(".so.tmp")
-            args = make(tmp)
-            jobs.append((target, tmp, args[0], subprocess.Popen(args, stderr=subprocess.PIPE, text=True)))
-    for target, tmp, compiler, process in jobs:
+    """Builds what is not up to date. The library needs no Torch, and is in place whatever becomes of the binding."""
+    jobs = []  # every command is put together before a compiler starts
+    if force or stale(TARGET, DEPENDS):
+        jobs.append((TARGET, TARGET.with_suffix(".so.tmp"), command(TARGET.with_suffix(".so.tmp"))))
+    tag = built_for()
+    if tag is None:
+        if verbose:
+            print("no Torch with CUDA: the binding of the operators on its tensors is left out", file=sys.stderr)
+    elif force or stale(TENSORS, [TENSORS_SOURCE, *DEPENDS[-1:]]) or tag.encode() not in TENSORS.read_bytes():
+        jobs.append((TENSORS, TENSORS.with_suffix(".so.tmp"), tensors_command(TENSORS.with_suffix(".so.tmp"))))
+    running, failures = [], []
+    for target, tmp, args in jobs:
+        try:
+            running.append((target, tmp, args, subprocess.Popen(args, stderr=subprocess.PIPE, text=True)))
+        except OSError as error:
+            failures.append(f"{Path(args[0]).name} failed:\n{error}")
+    for target, tmp, args, process in running:
         _, messages = process.communicate()
         if process.returncode:
-            raise RuntimeError(f"{Path(compiler).name} failed:\n{messages}")
+            failures.append(f"{Path(args[0]).name} failed:\n{messages}")
+            tmp.unlink(missing_ok=True)
+            continue
         if verbose and messages:
             print(messages, file=sys.stderr)
         os.replace(tmp, target)
+    if failures:
+        raise RuntimeError("\n".join(failures))
     return TARGET
 
 

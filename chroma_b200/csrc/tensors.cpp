@@ -350,4 +350,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensors", nullptr, -1, methods, n
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__tensors() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__tensors() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "built_for", BUILT_FOR) < 0) Py_CLEAR(m);
+    return m;
+}
