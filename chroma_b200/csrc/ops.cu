@@ -108,6 +108,16 @@ int sm_count() {
     return n;
 }
 
+// Lets a kernel have up to `bytes` of dynamic shared memory, the most that any call of it asks for: set once per device, so that no
+// call takes away what another thread's has been given.
+template <auto Kernel> void allow_smem(size_t bytes) {
+    static std::atomic<bool> done[kDevices];
+    const int device = current_device();
+    if (device < kDevices && done[device].load(std::memory_order_acquire)) return;
+    check(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)), "smem attribute");
+    if (device < kDevices) done[device].store(true, std::memory_order_release);
+}
+
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 constexpr int kMaxRows = 1 << 30;  // positions of a slot: row numbers stay well inside 32 bits
@@ -378,14 +388,15 @@ void copy_pages(const chroma_b200_pages& p, const int* list, const int* count, c
 
 // One CTA decides about pages and slots that fit its shared memory, and a table that it reads in a few rounds (4,096 pages:
 // compaction 177 us and a step with forks 18, by events around a graph; with several launches 182 and 20).
+constexpr int kOneCtaPages = 32 * 1024, kOneCtaSlots = 1024;
 bool one_cta(const chroma_b200_pages& p) {
-    return p.pages <= 32 * 1024 && p.slots <= 1024 && int64_t(p.slots) * p.width <= 64 * 1024;
+    return p.pages <= kOneCtaPages && p.slots <= kOneCtaSlots && int64_t(p.slots) * p.width <= 64 * 1024;
 }
 
-template <typename K> size_t shared_marks(K kernel, const chroma_b200_pages& p) {
-    const size_t bytes = size_t(p.pages) * 4 + size_t(p.slots) * sizeof(SlotStep) + size_t(p.pages) * 2;
-    if (bytes > 48 * 1024) check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)), "smem attribute");
-    return bytes;
+size_t marks_bytes(int pages, int slots) { return size_t(pages) * 4 + size_t(slots) * sizeof(SlotStep) + size_t(pages) * 2; }
+template <auto Kernel> size_t shared_marks(const chroma_b200_pages& p) {
+    allow_smem<Kernel>(marks_bytes(kOneCtaPages, kOneCtaSlots));
+    return marks_bytes(p.pages, p.slots);
 }
 
 // Bytes of the best of every segment of every row: of k_logits, or of k_logits_rest and k_logits_heard.
@@ -419,7 +430,7 @@ void step_pages(const chroma_b200_pages* p, const int32_t* parents, const int32_
     a.copies = a.free_list + p->pages;
     a.slots = p->slots, a.width = p->width, a.pages = p->pages, a.page = p->page_rows;
     a.cut = cut;
-    if (one_cta(*p)) launch(s, dim3(1), dim3(1024), shared_marks(k_pages_step, *p), k_pages_step, a);
+    if (one_cta(*p)) launch(s, dim3(1), dim3(1024), shared_marks<k_pages_step>(*p), k_pages_step, a);
     else {
         check(cudaMemsetAsync(a.keeper, 0, size_t(p->pages) * 4, s), "memset");
         launch(s, table_grid(*p), dim3(256), 0, k_pages_gather, a);
@@ -546,7 +557,7 @@ int chroma_b200_compact_pages(const chroma_b200_pages* p, int32_t* new_table, in
         a.copies = static_cast<int*>(workspace) + p->pages;
         a.holes = a.copies + 3 * p->pages + 1;
         a.slots = p->slots, a.width = p->width, a.pages = p->pages, a.page = p->page_rows;
-        if (one_cta(*p)) launch(s, dim3(1), dim3(1024), shared_marks(k_compact, *p), k_compact, a);
+        if (one_cta(*p)) launch(s, dim3(1), dim3(1024), shared_marks<k_compact>(*p), k_compact, a);
         else {
             check(cudaMemsetAsync(a.held, 0, size_t(p->pages) * 4, s), "memset");
             launch(s, table_grid(*p), dim3(256), 0, k_compact_mark, a);
@@ -604,7 +615,7 @@ int chroma_b200_process_logits(const chroma_b200_logits* g, void* stream, char* 
             a.best_at = long_segments;
             a.segments += ctas;
             const int smem = int(sizeof(HeardTable)) + (a.special_stride + ctas - 1) / ctas * 4;
-            check(cudaFuncSetAttribute(k_logits_heard<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "smem attribute");
+            allow_smem<k_logits_heard<T>>(sizeof(HeardTable) + kHeardWords * 4);
             launch(s, dim3(unsigned(ctas), unsigned(g->rows)), dim3(kHeardThreads), smem, k_logits_heard<T>, a);
             launch_after(s, rest, threads, k_logits_rest<T>, a);
         });
