@@ -15,7 +15,8 @@ sequence (below 0: none); and int32 ``lengths [slots]``, the rows that each hold
 
 Pools may have any strides that are multiples of 16 bytes (a layer of a larger pool, keys and values side by side); a
 head's row is contiguous and a multiple of 16 bytes. Everything is queued on the current stream of the tensors' device;
-nothing waits for the device or reads it from the host (``check_operators`` does). Wrong arguments raise ``ValueError``
+nothing waits for the device or reads it from the host (``check_operators`` does). No operator has a gradient: an output of
+tensors that want one raises when it is differentiated, and nothing passes through the cache. Wrong arguments raise ``ValueError``
 (``TypeError`` for what is not a tensor). The binding is ``chroma_b200/csrc/tensors.cpp``.
 """
 

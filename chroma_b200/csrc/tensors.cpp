@@ -12,6 +12,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -77,6 +79,34 @@ struct Call {
     void* stream() const { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
     Tensor empty(at::IntArrayRef shape, at::ScalarType type) const { return at::empty(shape, at::TensorOptions().dtype(type).device(device)); }
 };
+
+// The operators have no gradients. What comes of a tensor that wants one says so when it is differentiated; what is written in
+// place counts its version up, so that a graph which still needs the old values says so.
+using Inputs = std::initializer_list<const Tensor*>;
+bool wanted(Inputs inputs) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : inputs)
+        if (t && t->requires_grad()) return true;
+    return false;
+}
+void no_gradient(const char* name, Inputs inputs, Inputs outputs) {
+    if (!wanted(inputs)) return;
+    for (const Tensor* out : outputs) {
+        if (!out->defined()) continue;
+        torch::autograd::edge_list edges;
+        for (const Tensor* t : inputs)
+            if (t && t->requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(*t));
+        std::shared_ptr<torch::autograd::Node> node(new torch::autograd::NotImplemented(name), torch::autograd::deleteNode);
+        node->set_next_edges(std::move(edges));
+        torch::autograd::set_history(*out, node);
+    }
+}
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void check_out(const Tensor* out, Inputs inputs) {
+    TORCH_CHECK_VALUE(!out || !(wanted(inputs) || wanted({out})), "out cannot be given where a gradient is wanted (torch.no_grad() turns them off)");
+}
 
 void run(int status, const char* err) {
     TORCH_CHECK_VALUE(status != CHROMA_B200_VALUE, err);
@@ -144,6 +174,7 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     char err[512];
     run(native.paged_append(&p, nk.const_data_ptr(), nv.const_data_ptr(), strides, ints(call, starts, int64_t(p.slots) + 1, "starts"),
                             int32_t(nk.size(0)), call.stream(), err, sizeof err), err);
+    written(keys), written(tensor(args[1], "values"));
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -166,6 +197,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     g.window = integer(args[7], "window");
     g.first = integer(args[8], "first");
     const int lse = PyObject_IsTrue(args[10]);
+    const Inputs inputs = {&q, &keys, &tensor(args[2], "values"), sinks};
+    check_out(given, inputs);
     if (given) {
         call.with(given);
         TORCH_CHECK_VALUE(given->sizes() == q.sizes() && given->scalar_type() == q.scalar_type(), "out must be ", q.sizes(), " ", q.scalar_type(),
@@ -199,6 +232,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     char err[512];
     run(native.paged_attention(&p, &g, call.stream(), err, sizeof err), err);
+    if (given) written(out);
+    no_gradient("paged_attention", inputs, {&out, &logs});
     return lse ? Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(logs)) : THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }
@@ -217,6 +252,7 @@ PyObject* step_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int cut = truth(args[6]);
     run((cut ? native.step_pages : native.step_pages_uncut)(&p, parents, counts, new_table.data_ptr<int32_t>(), new_lengths.data_ptr<int32_t>(), info.data_ptr<int32_t>(),
                           workspace.data_ptr(), room, call.stream(), err, sizeof err), err);
+    written(keys), written(tensor(args[5], "values"));
     return Py_BuildValue("(NNN)", THPVariable_Wrap(new_table), THPVariable_Wrap(new_lengths), THPVariable_Wrap(info));
     END_HANDLE_TH_ERRORS
 }
@@ -231,6 +267,7 @@ PyObject* compact_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor new_table = call.empty({p.slots, p.width}, at::kInt), info = call.empty({2}, at::kInt), workspace = call.empty({room}, at::kByte);
     char err[512];
     run(native.compact_pages(&p, new_table.data_ptr<int32_t>(), info.data_ptr<int32_t>(), workspace.data_ptr(), room, call.stream(), err, sizeof err), err);
+    written(keys), written(tensor(args[3], "values"));
     return Py_BuildValue("(NN)", THPVariable_Wrap(new_table), THPVariable_Wrap(info));
     END_HANDLE_TH_ERRORS
 }
@@ -267,6 +304,8 @@ PyObject* process_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     TORCH_CHECK_VALUE(logits.dim() == 2 && logits.size(1) > 0 && logits.stride(1) == 1 && logits.size(0) <= INT32_MAX && logits.size(1) <= INT32_MAX,
                       "logits must be [rows, vocab] with contiguous rows, got ", logits.sizes());
     const int64_t rows = logits.size(0), vocab = logits.size(1);
+    const Inputs inputs = {&logits, t[4], t[5], t[6], bias, t[10]};
+    check_out(given, inputs);
     if (given) {
         call.with(given);
         TORCH_CHECK_VALUE(given->sizes() == logits.sizes() && given->scalar_type() == logits.scalar_type() && given->stride(1) == 1 &&
@@ -311,6 +350,8 @@ PyObject* process_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     char err[512];
     run(native.process_logits(&g, call.stream(), err, sizeof err), err);
+    if (given) written(out);
+    no_gradient("process_logits", inputs, {&out});
     // `out` comes back as the object that was given.
     PyObject* result = given ? Py_NewRef(args[11]) : THPVariable_Wrap(out);
     return argmax ? Py_BuildValue("(NN)", result, THPVariable_Wrap(best)) : result;
