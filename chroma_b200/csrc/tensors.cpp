@@ -48,7 +48,7 @@ const Tensor* optional(PyObject* o, const char* name) { return o == Py_None ? nu
 int integer(PyObject* o, const char* name) {
     const long v = PyLong_AsLong(o);
     if (v == -1 && PyErr_Occurred()) throw python_error();
-    TORCH_CHECK_VALUE(v >= 0 && v <= INT32_MAX, name, " must be nonnegative, got ", v);
+    TORCH_CHECK_VALUE(v >= 0 && v <= INT32_MAX, name, " must be nonnegative and below 2^31, got ", v);
     return int(v);
 }
 
@@ -196,7 +196,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (PyErr_Occurred()) throw python_error();
     g.window = integer(args[7], "window");
     g.first = integer(args[8], "first");
-    const int lse = PyObject_IsTrue(args[10]);
+    const bool lse = truth(args[10]);
     const Inputs inputs = {&q, &keys, &tensor(args[2], "values"), sinks};
     check_out(given, inputs);
     if (given) {
@@ -249,7 +249,7 @@ PyObject* step_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor new_table = call.empty({p.slots, p.width}, at::kInt), new_lengths = call.empty({p.slots}, at::kInt), info = call.empty({3}, at::kInt),
                  workspace = call.empty({room}, at::kByte);
     char err[512];
-    const int cut = truth(args[6]);
+    const bool cut = truth(args[6]);
     run((cut ? native.step_pages : native.step_pages_uncut)(&p, parents, counts, new_table.data_ptr<int32_t>(), new_lengths.data_ptr<int32_t>(), info.data_ptr<int32_t>(),
                           workspace.data_ptr(), room, call.stream(), err, sizeof err), err);
     written(keys), written(tensor(args[5], "values"));
@@ -338,7 +338,7 @@ PyObject* process_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
         g.mask = mask->const_data_ptr<int32_t>();
     }
     Tensor best, room;
-    const int argmax = PyObject_IsTrue(args[12]);
+    const bool argmax = truth(args[12]);
     if (argmax) {
         best = call.empty({rows}, at::kLong);
         g.argmax = best.data_ptr<int64_t>();

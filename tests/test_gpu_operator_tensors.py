@@ -69,3 +69,16 @@ def test_what_is_written_counts_its_version(gpu) -> None:  # type: ignore[no-unt
         pool = torch.zeros(3, 16, 2, 64, device="cuda", dtype=B16)
         chroma_b200.paged_append(pool, pool.clone(), q[:, :2], q[:, :2], table, n)
     chroma_b200.paged_append(pool, pool.clone(), q[:, :2], q[:, :2], table, n)
+
+
+def test_flags_that_are_neither_true_nor_false(gpu) -> None:  # type: ignore[no-untyped-def]
+    k, v, table, n = cache([20, 3], dtype=B16, kv=2, dim=64, page=16)
+    flag = torch.ones(2, dtype=torch.bool)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        chroma_b200.paged_attention(queries(2, 8, 64, B16), k, v, table, n, lse=flag)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        chroma_b200.process_logits(torch.randn(2, 100, device="cuda"), argmax=flag)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        chroma_b200.step_pages(table, n, n, n, k, v, cut=flag)
+    with pytest.raises(ValueError, match="below 2"):
+        chroma_b200.paged_attention(queries(2, 8, 64, B16), k, v, table, n, window=2**31)
