@@ -251,3 +251,54 @@ def test_bad_values_in_a_long_cache(gpu, what, heads, kv, dim, new) -> None:  # 
     assert torch.equal(got[away & ~hit], clean[away & ~hit])
     # 20 times and 5 ms: what is looked at again costs a pass over the values, not one over the cache for every row
     assert longer <= 20 * usual + 5
+
+
+# ---- many slots, many tiles, tables far wider than what is held
+
+@pytest.mark.parametrize("heads,kv,dim,page,slots,window", [
+    (8, 1, 64, 16, 90, 0),      # more than 64 sequences of a tile or two, one of many: the keys are not split
+    (16, 1, 128, 16, 90, 20), (40, 2, 64, 24, 70, 0), (3, 3, 80, 7, 130, 9),
+])
+def test_prompts_of_many_sequences(gpu, heads, kv, dim, page, slots, window) -> None:  # type: ignore[no-untyped-def]
+    new = [(s * 7) % 40 if s != 11 else 500 for s in range(slots)]
+    prior = [(s * 13) % 50 if s % 3 else 0 for s in range(slots)]
+    k, v, table, n = cache([a + b for a, b in zip(new, prior)], dtype=B16, kv=kv, dim=dim, page=page)
+    starts = torch.tensor([sum(new[:s]) for s in range(slots + 1)], dtype=torch.int32).cuda()
+    q = queries(sum(new), heads, dim, B16)
+    s = sink_values(heads, B16)
+    want = ref.attention(q, k, v, table, n, starts, scale=dim**-0.5, window=window, first=window // 5, sinks=s)
+    got, logs = chroma_b200.paged_attention(q, k, v, table, n, starts, window=window, first=window // 5, sinks=s, lse=True)
+    check(got, want, dtype=B16, dim=dim, lse=logs)
+
+
+def test_prompts_of_more_than_1024_tiles(gpu) -> None:  # type: ignore[no-untyped-def]
+    # 128 heads to a key-value head: two tokens a tile pair, 1,030 pairs in two sequences.
+    new, prior = [2000, 60], [0, 100]
+    k, v, table, n = cache([a + b for a, b in zip(new, prior)], dtype=B16, kv=1, dim=64, page=64)
+    starts = torch.tensor([0, 2000, 2060], dtype=torch.int32).cuda()
+    q = queries(2060, 128, 64, B16)
+    got, logs = chroma_b200.paged_attention(q, k, v, table, n, starts, window=50, first=3, lse=True)
+    for rows, positions in ((slice(0, 30), 0), (slice(990, 1020), 990), (slice(1970, 2000), 1970)):  # of the first sequence
+        part = torch.tensor([0, 30], dtype=torch.int32).cuda()
+        want = ref.attention(q[rows], k, v, table[:1], n[:1] * 0 + positions + 30, part, scale=0.125, window=50, first=3)
+        check(got[rows], want, dtype=B16, dim=64, lse=logs[rows])
+    want = ref.attention(q[2000:], k, v, table[1:], n[1:], torch.tensor([0, 60], dtype=torch.int32).cuda(), scale=0.125, window=50, first=3)
+    check(got[2000:], want, dtype=B16, dim=64, lse=logs[2000:])
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,page", [
+    (F32, 8, 1, 16, 16), (F32, 8, 2, 64, 32), (B16, 64, 8, 64, 64), (B16, 8, 2, 128, 16), (B16, 8, 1, 32, 16), (B16, 6, 2, 80, 5),
+])
+@pytest.mark.parametrize("window,first", [(0, 0), (100, 4)])
+def test_wide_tables(gpu, dtype, heads, kv, dim, page, window, first) -> None:  # type: ignore[no-untyped-def]
+    """What is seen of short sequences does not depend on how many positions their table could name."""
+    new, lengths = [5, 61, 0, 1, 30], [160, 98, 7, 1, 30]
+    k, v, table, n = cache(lengths, dtype=dtype, kv=kv, dim=dim, page=page)
+    wide = torch.full((5, 131072 // page), -1, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    s = sink_values(heads, F32)
+    for starts in (None, torch.tensor([0, 5, 66, 66, 67, 97], dtype=torch.int32).cuda()):
+        q = queries(sum(new) if starts is not None else 5, heads, dim, dtype)
+        want = ref.attention(q, k, v, table, n, starts, scale=0.2, window=window, first=first, sinks=s)
+        got, logs = chroma_b200.paged_attention(q, k, v, wide, n, starts, scale=0.2, window=window, first=first, sinks=s, lse=True)
+        check(got, want, dtype=dtype, dim=dim, lse=logs)
