@@ -82,7 +82,11 @@ def paged_attention(q: Tensor, keys: Tensor, values: Tensor, table: Tensor, leng
 
     Returns the output in q's type, and with ``lse`` the fp32 ``[tokens, heads]`` logarithms of the sums, by which parts
     of an attention can be joined. A token that sees nothing gives zeros and its sink (or -inf). Non-finite values in
-    rows that a token does not see do not reach it.
+    rows that a token does not see do not reach it. A token past the end of the table sees what has pages.
+
+    In float32 everything is held in 32 bits. In bfloat16 so are scores, sums and the running maximum, but the softmax's
+    weights go into the product with the values as bfloat16, as the tensor cores take them: against 64 bits the relative
+    error of a result is about 2.2e-3, where rounding the result alone costs 1.7e-3.
     """
     return ops.paged_attention(q, keys, values, table, lengths, starts, scale, window, first, sinks, lse, out)
 

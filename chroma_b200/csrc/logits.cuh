@@ -11,8 +11,8 @@
 // Bound: one row by the latency of a few dependent reads (history of 500: 9 us one call after another, as long as the
 // host's call). 64 rows of 201,088 with histories of 50-4,096, 50 biases and a mask, fp32: 32 us, 3.2 TB/s, where the bytes
 // alone take 16: 8 us are the chain of row length, history, table, logits of the first launch, under which only the first
-// segments of the second are read, and the second one issues 20 instructions an entry (five of them the division by the temperature);
-// 128 rows 55 us. All in one launch, with segments of 4,096 to 16,384 entries on 128 to 1,024 threads, took 45 to 57 us for
+// segments of the second are read (its stores wait, which a call in place needs and another would not), and the second one
+// issues 20 instructions an entry (five of them the division by the temperature); 128 rows 55 us. All in one launch, with segments of 4,096 to 16,384 entries on 128 to 1,024 threads, took 45 to 57 us for
 // the 64 rows; a table with a place for each of 16,384 entries in place of the hash table 47.
 #pragma once
 

@@ -220,8 +220,9 @@ struct DecodeSpace {
         bytes = parts + ml + int64_t(grid) * 16;
     }
     // One CTA per item where its warps have one or two units anyway, where there are so many items that they even out,
-    // and where the heads alone outnumber the CTAs; prompts have an item per rows in fp32, and no cuts. (One sequence of
-    // 160 positions: 12 us by events around a graph; cut and joined 16.)
+    // and where the heads alone outnumber the CTAs; prompts have an item per rows in fp32, and no cuts. The host knows the
+    // positions that the table could name, not those that are held. (One sequence of 160 positions, 8/1 heads of 16: 8.4 us;
+    // cut and joined, as in a table for 131,072, 10.7.)
     bool whole(int slots, int kv, int64_t positions, const void* starts) const {
         return starts || positions <= 256 || int64_t(slots) * kv * blocks >= int64_t(8) * grid || int64_t(kv) * blocks > sm_count();
     }
@@ -298,7 +299,8 @@ void attention_fp32(const PagedArgs& a, const chroma_b200_attention& g, cudaStre
     p.whole = space.whole(a.slots, a.kv, int64_t(a.width) * a.page, a.starts);
     int64_t blocks = a.starts ? (int64_t(a.tokens) + per_item - 1) / per_item * lines : p.whole ? items : sm_count() * 2;
     // Items of a prompt that leave SMs without work share them out, as long as every warp may have two units (16 tokens after
-    // 8,000, 16/2 heads of 64: 47 us, without 174; after 4,000 with 64/8 heads 70 and 102).
+    // 8,000, 16/2 heads of 64: 47 us, without 174; after 4,000 with 64/8 heads 70 and 102). By the positions that the table could
+    // name: three prompts of 5-61 after 37, 8/1 heads of 16, take 8.6 us, and 12.5 in a table for 131,072.
     p.share = 1;
     if (a.starts)
         while (p.share < 8 && 2 * p.share * blocks <= 2 * sm_count() && int64_t(a.width) * a.page >= 2 * p.share * 2 * kF32Warps * 32) p.share *= 2;
@@ -327,7 +329,8 @@ struct PromptSpace {
     PromptSpace(int tokens, int group, int slots, int kv, int dim, int64_t positions) {
         tiles = int(int64_t(tokens) * group / 256) + std::max(1, std::min(slots, tokens));
         items = int64_t(tiles) * kv;
-        // Fewer items than half the SMs share the SMs out, as long as four key tiles are left to each split.
+        // Fewer items than half the SMs share the SMs out, as long as four key tiles of the positions that the table could name are
+        // left to each split. (Two prompts of 100, 64/8 heads of 64: 10.4 us; in a table for 131,072, with splits, 24.8.)
         const int64_t most = positions / (4 * kPrTile), share = sm_count() / items;
         if (share > 1 && most > 1) splits = int(share < most ? share : most);
         if (splits > 1) {
@@ -386,8 +389,10 @@ void copy_pages(const chroma_b200_pages& p, const int* list, const int* count, c
     launch_after(s, dim3(unsigned(columns), unsigned(parts)), dim3(256), k_pages_copy, a, list, count);
 }
 
-// One CTA decides about pages and slots that fit its shared memory, and a table that it reads in a few rounds (4,096 pages:
-// compaction 177 us and a step with forks 18, by events around a graph; with several launches 182 and 20).
+// One CTA decides about pages and slots that fit its shared memory, and a table that it reads in a few rounds. The decisions
+// alone, steps and compaction, with pages of 1 KB: 4,096 pages and 128 slots 10.7 and 12.8 us, with several launches 11.3 and 16.9;
+// 16,384 and 512: 25.1 and 39.4, 23.0 and 35.3; 32,768 and 1,000: 59.9 and 80.9, 57.4 and 70.1; 32,768 and 64: 44.0 and 33.3, 60.4 and
+// 41.5. So it loses where pools and slots are both large, by 4 to 15%, and wins elsewhere by as much or more.
 constexpr int kOneCtaPages = 32 * 1024, kOneCtaSlots = 1024;
 bool one_cta(const chroma_b200_pages& p) {
     return p.pages <= kOneCtaPages && p.slots <= kOneCtaSlots && int64_t(p.slots) * p.width <= 64 * 1024;

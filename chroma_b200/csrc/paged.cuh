@@ -1,5 +1,4 @@
-// A paged key-value cache: what its operators share, the write of new rows, and the attention of any token over the
-// pages of its sequence.
+// A paged key-value cache: what its operators share, and the write of new rows.
 //
 // Position p of slot s is row p % page of page table[s][p / page] of the pools. A token at position p sees position j
 // iff j <= p, j's page exists, and p - j < window or j < first (no window: every j <= p). All sums and the softmax's

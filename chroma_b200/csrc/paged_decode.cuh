@@ -321,8 +321,8 @@ template <int DC, int NT> struct DecodeRegs {
 // contraction of S runs over the dims in any order that K and Q share, and the columns of O may stand in any order, so
 // every operand is cut such that a lane's share of a K or V row is 16 contiguous bytes: lane (g, t) of a warp loads
 // dims 32 c + 8 t .. + 7 of keys g and g + 8 for S, and dims 64 d + 8 g .. + 7 of keys 2t, 2t + 1, 2t + 8, 2t + 9 for
-// O. It copies them with cp.async into slots of shared memory that only it reads, a ring of stages ahead, so the ring
-// needs no barrier at all. V's pairs of keys are put together with byte permutations, P is turned from the score
+// O. It loads them straight into registers, a unit ahead: the next unit's keys once this one's scores are done, its values
+// once this one's outputs are. V's pairs of keys are put together with byte permutations, P is turned from the score
 // layout into the operand layout by movmatrix.
 template <int DC, int NT, bool kAligned>
 __global__ void __launch_bounds__(32 * DecodeRegs<DC, NT>::kWarps, DecodeRegs<DC, NT>::kCtas)

@@ -10,12 +10,14 @@
 // are cut, merged and joined as in paged_decode.cuh. Few items of a prompt after a long cache are each shared by the CTAs of a
 // cluster, which merge through one another's shared memory.
 //
-// What bounds it: where caches are short, the latency of five dependent reads; else shared memory and its load instructions
-// (of 32 keys and 64 values: 1,024 FMA instructions a warp, and about 400 cycles of the SM's load pipe; with each lane reading
-// its own key from global memory, and weights passed by shuffles, it was 870). 64 sequences of 500-2,000 positions with 64/8
-// heads of 64: 109 us, 12 TFLOP/s (143 in that form); two of 30,000-60,000 with 8/2 heads of 128: 78 us; two prompts of 1,000
-// with 16/4 heads of 64: 297 us; 16 tokens after 8,000, 16/2 heads of 64: 47 us. One sequence of 160 with 8 heads of 16:
-// 7.7 us one call after another.
+// What bounds it: where caches are short, the latency of five dependent reads; else the latency of a unit's copies, which
+// nothing hides but the other warps. A warp waits for its keys as soon as it has asked for them, and reads the values after the
+// weights. 64 sequences of 500-2,000 positions with 64/8 heads of 64 take 109 us, 12 TFLOP/s, where their bytes take 51, the
+// load pipe's work (about 400 cycles of an SM for 32 keys and 64 values) 28 and the FMA's issue 18; with each lane reading its
+// own key from global memory, and weights passed by shuffles, they took 143. Two of 30,000-60,000 with 8/2 heads of 128: 78 us
+// (bytes 28); two prompts of 1,000 with 16/4 heads of 64: 301 us; 16 tokens after 8,000, 16/2 heads of 64: 47 us. One sequence of
+// 160 with 8 heads of 16: 8.2 us one call after another. At 128 registers, which let two CTAs share an SM, every width spills
+// (132 bytes stored, 88 loaded a thread).
 #pragma once
 
 #include <limits.h>

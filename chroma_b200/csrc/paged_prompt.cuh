@@ -22,11 +22,12 @@
 // What bounds it: the exponentials and what goes with them on 128 rows of one thread each, in turn with the products
 // (clock stamps per tile of 64-value heads: 1,400 cycles of exponentials, 650 around them, 1,000 waiting; the
 // special-function unit is busy half of the time, the tensor core a quarter). Four prompts of 2,048 tokens, 64/8 heads of
-// 64: 276 us, 498 TFLOP/s (266 one call after another); 8,192 tokens after 8,001 in a window of 4,096, 32/8 heads of 128:
-// 580 us, 949 TFLOP/s, and 633 once the GPU is at its power limit; two prompts of 4,096 with 32/8 heads of 128: 297 us.
+// 64: 283 us, 486 TFLOP/s (269 one call after another); 8,192 tokens after 8,001 in a window of 4,096, 32/8 heads of 128:
+// 586 us, 939 TFLOP/s, and 628 once the GPU is at its power limit; two prompts of 4,096 with 32/8 heads of 128: 297 us. No unit
+// is full: issue slots 36 and 29% (heads of 64, 128), the special-function unit 52 and 44%, the tensor core 25 and 44%.
 // Tried when those two took 300 and 586 us, and slower: a quarter to a half of the exponentials as a polynomial on the FMA
-// pipe (305 to 354 us; issue slots), the issuing warp taking whatever is ready first (301 and 653 us), a second issuing
-// warp (317 and 640 us), the two tiles' exponentials in turn (313 and 604 us).
+// pipe (305 to 354 us, though issue slots are not short; why was not found), the issuing warp taking whatever is ready first
+// (301 and 653 us), a second issuing warp (317 and 640 us), the two tiles' exponentials in turn (313 and 604 us).
 //
 // A position that no row may see costs nothing (whole tiles are passed over) or a mask of 128 bits per row, applied only
 // to the tiles that need it. Values behind the end of a sequence are cleared in shared memory, since what lies there may
@@ -46,8 +47,8 @@
 namespace cb200 {
 
 constexpr int kPrThreads = 384, kPrTile = 128;
+constexpr int kPrSorted = 1024, kPrSortedSlots = 64;  // pairs of tiles and slots that are put in order
 // Registers of a softmax thread and of the others, out of the 3 x 168 that three warpgroups are launched with.
-constexpr int kPrSorted = 1024, kPrSortedSlots = 64;  // tiles, slots
 constexpr int kPrSoftmaxRegs = 216, kPrOtherRegs = 72;
 
 // The products are issued by one elected thread of a converged warp: everything they need is the same in all lanes, so it
