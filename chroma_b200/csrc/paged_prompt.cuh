@@ -281,26 +281,33 @@ template <int H> __device__ __forceinline__ void add_cleaned(const PagedPromptAr
     const PagedArgs& a = p.a;
     const SecondLook<H> look(p, number, sorted);
     const PromptItem& w = look.w;
+    bool done = look.pos < 0;  // no row, or nothing but NaN
 #pragma unroll 1
     for (int t = 0; t < w.tiles; ++t) {
         const int t0 = w.key0(t);
         if (whole_tile(p, w, 0, t0) && (w.active == 1 || whole_tile(p, w, 1, t0))) continue;
 #pragma unroll 1
         for (int j = t0; j < t0 + kPrTile; ++j) {
+            if (__all_sync(0xffffffffu, done)) return;
+            int nans = 0;
             const int entry = int(a.by_page.div(uint32_t(j))), id = entry < a.width ? __ldg(a.table + w.slot * a.ts + entry) : -1;
             if (id < 0 || id >= a.pages) continue;
             const auto* v = static_cast<const __nv_bfloat16*>(a.v) + id * a.vp + (j - entry * a.page) * a.vr + w.kvh * a.vh;
 #pragma unroll 1
             for (int d = 0; d < a.dim; d += 8) {
-                if (!has_bad(__ldg(reinterpret_cast<const uint4*>(v + d))) || look.pos < 0 || !sees(look.pos, j, a.window, a.first)) continue;
+                if (!has_bad(__ldg(reinterpret_cast<const uint4*>(v + d))) || done || !sees(look.pos, j, a.window, a.first)) continue;
 #pragma unroll 1
                 for (int e = d; e < d + 8; ++e) {
                     const float x = __bfloat162float(v[e]);
                     if (x * 0.f == 0.f) continue;
-                    if (look.part) look.part[e] += x;
-                    else look.out[e] = __float2bfloat16_rn(__bfloat162float(look.out[e]) + x);
+                    nans += isnan(x);
+                    const float was = look.part ? look.part[e] : __bfloat162float(look.out[e]);
+                    if (was == x) continue;  // an infinity more
+                    if (look.part) look.part[e] = was + x;
+                    else look.out[e] = __float2bfloat16_rn(was + x);
                 }
             }
+            done = done || nans == a.dim;
         }
     }
 }

@@ -302,3 +302,17 @@ def test_wide_tables(gpu, dtype, heads, kv, dim, page, window, first) -> None:  
         want = ref.attention(q, k, v, table, n, starts, scale=0.2, window=window, first=first, sinks=s)
         got, logs = chroma_b200.paged_attention(q, k, v, wide, n, starts, scale=0.2, window=window, first=first, sinks=s, lse=True)
         check(got, want, dtype=dtype, dim=dim, lse=logs)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("heads,kv,dim,new,prior", [(16, 8, 64, 600, 3000), (8, 4, 128, 20, 6000)])
+def test_nothing_but_bad_values(gpu, bad, heads, kv, dim, new, prior) -> None:  # type: ignore[no-untyped-def]
+    k, v, table, n = cache([prior + new, new], dtype=B16, kv=kv, dim=dim, page=16, poison=False)
+    starts = torch.tensor([0, new, 2 * new], dtype=torch.int32).cuda()
+    q = queries(2 * new, heads, dim, B16)
+    clean = chroma_b200.paged_attention(q, k, v, table, n, starts)
+    v[table[0, : -(-(prior + new) // 16)].long()] = bad  # the first sequence's
+    got = chroma_b200.paged_attention(q, k, v, table, n, starts)
+    chroma_b200.check_operators()
+    assert torch.equal(got[new:], clean[new:])
+    assert bool((got[:new] == bad).all()) if bad == bad else bool(got[:new].isnan().all())
