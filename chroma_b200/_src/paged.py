@@ -81,7 +81,7 @@ def paged_attention(q: Tensor, keys: Tensor, values: Tensor, table: Tensor, leng
     (chroma/models/gpt_oss.py:133-151). ``scale`` is ``head_dim ** -0.5`` unless given.
 
     Returns the output in q's type, and with ``lse`` the fp32 ``[tokens, heads]`` logarithms of the sums, by which parts
-    of an attention can be joined. A token that sees nothing gives zeros and its sink (or -inf). Non-finite values in
+    of an attention can be joined. ``out`` may be ``q`` itself. A token that sees nothing gives zeros and its sink (or -inf). Non-finite values in
     rows that a token does not see do not reach it. A token past the end of the table sees what has pages.
 
     In float32 everything is held in 32 bits. In bfloat16 so are scores, sums and the running maximum, but the softmax's

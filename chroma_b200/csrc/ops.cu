@@ -376,6 +376,11 @@ void prompt(const PagedArgs& a, const chroma_b200_attention& g, int storage, cud
     p.error = error_word();
     const int64_t size = int64_t(element(storage));
     p.q_vector = aligned16(a.q) && a.qt * size % 16 == 0 && a.qh * size % 16 == 0;
+    // A result may be written over its query: each row's is read before, once.
+    const auto end = [&](const void* at, int64_t token, int64_t head) {
+        return reinterpret_cast<uintptr_t>(at) + ((a.tokens - 1) * token + (a.heads - 1) * head + a.dim) * size;
+    };
+    p.over_q = reinterpret_cast<uintptr_t>(a.q) < end(a.out, a.ot, a.oh) && reinterpret_cast<uintptr_t>(a.out) < end(a.q, a.qt, a.qh);
     p.out_vector = aligned16(a.out) && a.ot * size % 16 == 0 && a.oh * size % 16 == 0;
     if (a.dim <= 64) prompt_bf16<1>(p, g, s);
     else prompt_bf16<2>(p, g, s);

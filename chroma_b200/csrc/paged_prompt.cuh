@@ -105,6 +105,7 @@ struct PagedPromptArgs {
     int box;                 // rows of a TMA box; 0: row by row
     int q_vector, out_vector;  // rows are 16-byte aligned
     int q_box;               // Q tiles come as one TMA box: `group` heads of 128 / group tokens
+    int over_q;              // results are written over Q: no second time, the first is taken like it
     int tiles;               // pairs of tiles of rows at most: what the workspace has room for
     int splits;              // of the keys of an item, where there are few items
     FastDiv by_splits;
@@ -139,7 +140,7 @@ __device__ __forceinline__ uint32_t* prompt_order() {
 struct PromptCursor {
     int slot, before, round;  // tiles of the slots after `slot`
     bool sorted;              // or prompt_order() has slot << 16 | tile of each place
-    bool second = false;      // the second time
+    bool second = false;      // the second time, or the only one
     __device__ __forceinline__ explicit PromptCursor(const PagedArgs& a, bool in_order = false)
         : slot(a.slots - 1), before(0), round(0), sorted(in_order) {}
     // The end of the first time, for every warp of the CTA.
@@ -385,6 +386,7 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
 
     if (warp >= 8) {
     PromptCursor cursor(a, sorted);
+    cursor.second = p.over_q;
     PromptItem w;
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrOtherRegs));
     if (warp == 9) {
@@ -583,6 +585,7 @@ k_paged_prompt(const __grid_constant__ PagedPromptArgs p, const __grid_constant_
         const uint32_t tP = kOwnP ? tmem + uint32_t(2 * kPrTile + k * 64) + lanes : tS;
         int g = 0, uses = 0, ends = 0;
         PromptCursor cursor(a, sorted);
+        cursor.second = p.over_q;
         PromptItem w;
         while (!abort_flag) {
             if (!cursor.next(p, total, w)) {

@@ -263,7 +263,7 @@ int chroma_b200_paged_append(const chroma_b200_pages* pages, const void* new_key
 
 typedef struct chroma_b200_attention {
     const void *q;                /* [tokens][heads][head_dim] in the pools' storage */
-    void *out;                    /* the same shape and type */
+    void *out;                    /* the same shape and type; may be q itself */
     float *lse;                   /* [tokens][heads] or NULL */
     const void *sinks;            /* [heads] or NULL: one more term of the softmax's sum, with no value */
     const int32_t *starts;        /* [slots + 1], or NULL: one token per slot */
@@ -280,7 +280,8 @@ typedef struct chroma_b200_attention {
 /* out = softmax(scale q.K^T) V of each token over the positions it sees. Token i of slot b is at position
  * p = lengths[b] - tokens of b + i (which may lie past the table) and sees j <= p with p - j < window or j < first. The attention of
  * chroma/models/gpt_oss.py:133-151 (learned sinks, sliding window) over pages; `lse` is the logarithm of the sum. A
- * token that sees nothing gives zeros, and its sink (or -inf) as lse. */
+ * token that sees nothing gives zeros, and its sink (or -inf) as lse. Values that are not finite do not reach tokens that do
+ * not see them. */
 int chroma_b200_paged_attention(const chroma_b200_pages* pages, const chroma_b200_attention* args, void* stream,
                                 char* err, size_t err_len);
 /* Bytes of workspace that this call wants on the current device (0: none; -1: wrong arguments); its pointers are not

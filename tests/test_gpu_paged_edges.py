@@ -316,3 +316,41 @@ def test_nothing_but_bad_values(gpu, bad, heads, kv, dim, new, prior) -> None:  
     chroma_b200.check_operators()
     assert torch.equal(got[new:], clean[new:])
     assert bool((got[:new] == bad).all()) if bad == bad else bool(got[:new].isnan().all())
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,new,prior", [
+    (B16, 16, 8, 64, 600, 300), (B16, 8, 2, 128, 20, 3000), (B16, 200, 1, 64, 40, 30), (F32, 8, 2, 64, 90, 30), (F32, 8, 1, 16, 5, 4000),
+])
+def test_results_over_their_queries(gpu, dtype, heads, kv, dim, new, prior) -> None:  # type: ignore[no-untyped-def]
+    k, v, table, n = cache([prior + new, new], dtype=dtype, kv=kv, dim=dim, page=16, poison=False)
+    starts = torch.tensor([0, new, 2 * new], dtype=torch.int32).cuda()
+    for bad in (False, True):
+        if bad:
+            p = prior + new // 2
+            v[table[0, p // 16], p % 16, :, 3] = float("nan")
+        for s, rows in ((starts, 2 * new), (None, 2)):
+            for parts in (1, 3):  # queries of their own, and the first of what a projection gave
+                q = queries(rows, parts * heads, dim, dtype)[:, :heads]
+                want, logs = chroma_b200.paged_attention(q, k, v, table, n, s, lse=True)
+                got, again = chroma_b200.paged_attention(q, k, v, table, n, s, lse=True, out=q)
+                assert got.data_ptr() == q.data_ptr()
+                assert torch.equal(got.nan_to_num(9), want.nan_to_num(9)) and torch.equal(again, logs)
+    chroma_b200.check_operators()
+
+
+def test_results_over_their_queries_through_the_c_entry(gpu) -> None:  # type: ignore[no-untyped-def]
+    new, prior = 600, 300
+    k, v, table, n = cache([prior + new, new], dtype=B16, kv=8, dim=64, page=16, poison=False)
+    starts = torch.tensor([0, new, 2 * new], dtype=torch.int32).cuda()
+    q = queries(2 * new, 16, 64, B16)
+    p = prior + new // 2
+    v[table[0, p // 16], p % 16, :, 3] = float("nan")
+    want = chroma_b200.paged_attention(q, k, v, table, n, starts)
+    pages = pages_struct(k, v, table, n)
+    g = Attention(q.data_ptr(), q.data_ptr(), None, None, starts.data_ptr(), None, 0, (ctypes.c_int64 * 2)(1024, 64),
+                  (ctypes.c_int64 * 2)(1024, 64), 2 * new, 16, 0, 0, 0, 0.125)
+    g.workspace_bytes = nat.lib().chroma_b200_attention_workspace(ctypes.byref(pages), ctypes.byref(g))
+    room = torch.empty(max(1, g.workspace_bytes), dtype=torch.uint8, device="cuda")
+    g.workspace = room.data_ptr()
+    nat.call("chroma_b200_paged_attention", ctypes.byref(pages), ctypes.byref(g), torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(q.nan_to_num(9), want.nan_to_num(9))
