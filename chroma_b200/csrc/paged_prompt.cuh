@@ -23,7 +23,7 @@
 // (clock stamps per tile of 64-value heads: 1,400 cycles of exponentials, 650 around them, 1,000 waiting; the
 // special-function unit is busy half of the time, the tensor core a quarter). Four prompts of 2,048 tokens, 64/8 heads of
 // 64: 283 us, 486 TFLOP/s (269 one call after another); 8,192 tokens after 8,001 in a window of 4,096, 32/8 heads of 128:
-// 586 us, 939 TFLOP/s, and 628 once the GPU is at its power limit; two prompts of 4,096 with 32/8 heads of 128: 297 us. No unit
+// 586 us, 939 TFLOP/s, and 628 to 636 once the GPU is at its power limit; two prompts of 4,096 with 32/8 heads of 128: 297 us. No unit
 // is full: issue slots 36 and 29% (heads of 64, 128), the special-function unit 52 and 44%, the tensor core 25 and 44%.
 // Tried when those two took 300 and 586 us, and slower: a quarter to a half of the exponentials as a polynomial on the FMA
 // pipe (305 to 354 us, though issue slots are not short; why was not found), the issuing warp taking whatever is ready first
